@@ -1,5 +1,5 @@
 """Memory-bound ops (``csrc/kernels/elementwise.cu``): norms with fused residual add, activation
-backward, bias gradient, embedding, QK-norm + RoPE on packed QKV, LSE merge.
+backward, bias gradient, embedding, QK-norm + RoPE on packed QKV, LSE merge, dropout.
 
 Each public function takes CUDA bf16 tensors and launches our kernel, or CPU tensors and runs the
 PyTorch reference (oracle path).  Parameters that carry ``main_grad`` get their gradients
@@ -7,7 +7,7 @@ accumulated there in fp32.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -58,11 +58,78 @@ def add(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return y
 
 
+# ----------------------------------------------------------------------------- dropout
+class Dropout(NamedTuple):
+    """Which elements a dropout drops, and how many: a function of the seed, the site and an element's place, so that no mask is stored and
+    the same elements are dropped by the backward pass, by recomputed activations and by whatever rank holds them.
+
+    ``p``: share that is dropped, ``0 <= p < 1``; the others are divided by ``1 - p``.  ``seed``: one int64 on the tensor's device, which is
+    read there (a captured call takes what it holds at each replay) and may not change before the backward pass has run.  ``site``: a
+    number of the caller's for each place of a model that drops, below ``2**32``.  For ``x`` of ``[..., T, d]``, row ``t`` of sequence
+    ``b`` is drawn as row ``b * seq_len + pos[t]``: ``pos`` (int64 ``[T]``) are the global positions of a shard of sequences of ``seq_len``
+    tokens; without them the tensor holds whole sequences."""
+    p: float
+    seed: torch.Tensor
+    site: int = 0
+    pos: Optional[torch.Tensor] = None
+    seq_len: int = 0
+
+    def checked(self, x: torch.Tensor) -> "Dropout":
+        T = x.shape[-2] if x.dim() > 1 else 1
+        assert 0.0 <= self.p < 1.0, f"dropout: p={self.p} outside [0, 1)"
+        assert self.seed.dtype == torch.int64 and self.seed.numel() == 1 and self.seed.device == x.device, "dropout: the seed is one int64 on the tensor's device"
+        assert 0 <= self.site < 1 << 32, f"dropout: site {self.site} outside 32 bits"
+        if self.pos is not None:
+            assert self.pos.dtype == torch.int64 and self.pos.shape == (T,) and self.pos.device == x.device, "dropout: pos is int64 [T] on the tensor's device"
+            assert self.seq_len >= T, f"dropout: {T} positions of sequences of {self.seq_len}"
+        else:
+            assert self.seq_len in (0, T), f"dropout: {T} rows of sequences of {self.seq_len} need their positions"
+        return self._replace(seq_len=self.seq_len or max(1, T), pos=None if self.pos is None else self.pos.contiguous())
+
+    def _args(self, shape) -> tuple:
+        """What the launchers take; ``checked`` has been called."""
+        return self.seed.data_ptr(), nv.ptr(self.pos), shape[-2] if len(shape) > 1 else 1, self.seq_len, self.site, float(self.p)
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, seed, pos, drop):
+        ctx.save_for_backward(seed, pos)
+        ctx.drop = drop._replace(seed=None, pos=None)
+        return _dropout(x, drop)
+
+    @staticmethod
+    def backward(ctx, dy):
+        seed, pos = ctx.saved_tensors
+        return _dropout(dy, ctx.drop._replace(seed=seed, pos=pos)), None, None, None
+
+
+def _dropout(x: torch.Tensor, drop: Dropout) -> torch.Tensor:
+    x2 = x.contiguous()
+    if x2.data_ptr() % 16:
+        x2 = x2.clone()
+    y = torch.empty_like(x2)
+    d = x.shape[-1]
+    nv.call("dropout", x2.data_ptr(), y.data_ptr(), x2.numel() // max(1, d), d, *drop._args(x.shape), nv.stream_ptr(x.device))
+    return y
+
+
+def dropout(x: torch.Tensor, drop: Dropout) -> torch.Tensor:
+    """``x / (1 - p)`` where an element is kept, 0 where it is dropped (whatever it holds)."""
+    drop = drop.checked(x)
+    if drop.p == 0.0:
+        return x
+    if x.is_cuda:
+        assert x.dtype == torch.bfloat16, f"the kernels compute in bf16 (got {x.dtype})"
+        return _DropoutFn.apply(x, drop.seed, drop.pos, drop)
+    return ref.dropout(x, drop)
+
+
 # ----------------------------------------------------------------------------- norms
 class _NormFn(torch.autograd.Function):
     """``y = norm(x [+ res])``; returns ``(y, x_new)`` where ``x_new = x + res`` (or ``x``)."""
     @staticmethod
-    def forward(ctx, x, res, w, b, eps, layer):
+    def forward(ctx, x, res, w, b, eps, layer, drop=None):
         d = x.shape[-1]
         x2 = x.reshape(-1, d)
         if not x2.is_contiguous():
@@ -77,17 +144,23 @@ class _NormFn(torch.autograd.Function):
             xnew = torch.empty_like(x2)
         else:
             r2, xnew = None, x2
-        nv.call("norm_fwd", nv.ptr(x2), nv.ptr(r2), nv.ptr(w), nv.ptr(b), nv.ptr(xnew), nv.ptr(y), nv.ptr(stats),
-                nv.i(rows), nv.i(d), nv.f(eps), nv.i(layer), nv.stream_ptr(x.device))
-        ctx.save_for_backward(xnew, stats)
+        if drop is None:
+            nv.call("norm_fwd", nv.ptr(x2), nv.ptr(r2), nv.ptr(w), nv.ptr(b), nv.ptr(xnew), nv.ptr(y), nv.ptr(stats),
+                    nv.i(rows), nv.i(d), nv.f(eps), nv.i(layer), nv.stream_ptr(x.device))
+            ctx.save_for_backward(xnew, stats)
+        else:
+            nv.call("norm_drop_fwd", x2.data_ptr(), r2.data_ptr(), nv.ptr(w), nv.ptr(b), xnew.data_ptr(), y.data_ptr(), stats.data_ptr(), rows, d,
+                    eps, layer, *drop._args(x.shape), nv.stream_ptr(x.device))
+            ctx.save_for_backward(xnew, stats, drop.seed, drop.pos)
         ctx.w, ctx.b, ctx.layer, ctx.has_res = w, b, layer, res is not None
+        ctx.drop = None if drop is None else drop._replace(seed=None, pos=None)
         ctx.shape = x.shape
         ctx.set_materialize_grads(False)
         return y.view(x.shape), xnew.view(x.shape)
 
     @staticmethod
     def backward(ctx, dy, dxnew):
-        xnew, stats = ctx.saved_tensors
+        xnew, stats, *key = ctx.saved_tensors
         w = ctx.w
         d = xnew.shape[-1]
         if dy is None:
@@ -109,32 +182,52 @@ class _NormFn(torch.autograd.Function):
             own_dw = dw_buf = torch.zeros(d, dtype=torch.float32, device=dy.device)
         if bp is not None and db_buf is None:
             own_db = db_buf = torch.zeros(d, dtype=torch.float32, device=dy.device)
-        nv.call("norm_bwd", nv.ptr(xnew), nv.ptr(dy2), nv.ptr(dres2), nv.ptr(w), nv.ptr(stats), nv.ptr(dx),
-                nv.ptr(dw_buf), nv.ptr(db_buf), nv.i(xnew.shape[0]), nv.i(d), nv.i(ctx.layer), nv.stream_ptr(dy.device))
+        if ctx.drop is None:
+            dbranch = dx
+            nv.call("norm_bwd", nv.ptr(xnew), nv.ptr(dy2), nv.ptr(dres2), nv.ptr(w), nv.ptr(stats), nv.ptr(dx),
+                    nv.ptr(dw_buf), nv.ptr(db_buf), nv.i(xnew.shape[0]), nv.i(d), nv.i(ctx.layer), nv.stream_ptr(dy.device))
+        else:
+            dbranch = torch.empty_like(xnew)
+            nv.call("norm_drop_bwd", xnew.data_ptr(), dy2.data_ptr(), nv.ptr(dres2), nv.ptr(w), stats.data_ptr(), dx.data_ptr(), dbranch.data_ptr(),
+                    nv.ptr(dw_buf), nv.ptr(db_buf), xnew.shape[0], d, ctx.layer,
+                    *ctx.drop._replace(seed=key[0], pos=key[1])._args(ctx.shape), nv.stream_ptr(dy.device))
         for prm in (wp, bp):
             hook = getattr(prm, "_grad_ready", None) if prm is not None else None
             if hook is not None:
                 hook(prm)
         dx = dx.view(ctx.shape)
-        return (dx, dx if ctx.has_res else None,
+        return (dx, dbranch.view(ctx.shape) if ctx.has_res else None,
                 None if own_dw is None else own_dw.to(wp.dtype), None if own_db is None else own_db.to(bp.dtype),
-                None, None)
+                None, None, None)
 
 
-def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None
-            ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Returns ``(rmsnorm(x + residual) * w, x + residual)``."""
+def _branch_drop(x: torch.Tensor, residual: Optional[torch.Tensor], drop: Optional[Dropout]) -> Optional[Dropout]:
+    """``drop`` as the norms take it: checked, None where nothing is dropped."""
+    if drop is None:
+        return None
+    assert residual is not None and residual.shape == x.shape, "a norm's dropout is that of its residual branch"
+    drop = drop.checked(x)
     if x.is_cuda:
-        return _NormFn.apply(x, residual, w, None, eps, 0)
-    xn = x if residual is None else x + residual
+        assert x.dtype == residual.dtype == torch.bfloat16, f"the kernels compute in bf16 (got {x.dtype} and {residual.dtype})"
+    return drop if drop.p else None
+
+
+def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None,
+            drop: Optional[Dropout] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Returns ``(rmsnorm(x + residual) * w, x + residual)``; with ``drop``, ``dropout(residual, drop)`` in the place of ``residual``."""
+    drop = _branch_drop(x, residual, drop)
+    if x.is_cuda:
+        return _NormFn.apply(x, residual, w, None, eps, 0, drop)
+    xn = x if residual is None else x + (residual if drop is None else ref.dropout(residual, drop))
     return ref.rmsnorm(xn, w, eps), xn
 
 
 def layernorm(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], eps: float,
-              residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+              residual: Optional[torch.Tensor] = None, drop: Optional[Dropout] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    drop = _branch_drop(x, residual, drop)
     if x.is_cuda:
-        return _NormFn.apply(x, residual, w, b, eps, 1)
-    xn = x if residual is None else x + residual
+        return _NormFn.apply(x, residual, w, b, eps, 1, drop)
+    xn = x if residual is None else x + (residual if drop is None else ref.dropout(residual, drop))
     return ref.layernorm(xn, w, b, eps), xn
 
 

@@ -41,6 +41,31 @@ def swiglu(gu: torch.Tensor) -> torch.Tensor:
     return (F.silu(g) * u).to(gu.dtype)
 
 
+# ----------------------------------------------------------------------------- dropout
+def philox(row: torch.Tensor, columns: int, site: int, seed: torch.Tensor) -> torch.Tensor:
+    """Words of Philox4x32 with seven rounds (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) as int64
+    ``[rows, columns]``: counter ``(column // 4, row, row >> 32, site)``, key ``seed``, a word for each of four columns."""
+    low = 0xffffffff
+    c0 = torch.arange((columns + 3) // 4, device=row.device).expand(row.numel(), -1)
+    c1, c2, c3 = (row & low)[:, None].expand_as(c0), (row >> 32 & low)[:, None].expand_as(c0), torch.full_like(c0, site)
+    k0, k1 = seed.reshape(()) & low, seed.reshape(()) >> 32 & low
+    for _ in range(7):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57             # int64 keeps the product's 64 bits, the masks drop its sign
+        c0, c1, c2, c3 = (b >> 32 & low) ^ c1 ^ k0, b & low, (a >> 32 & low) ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    return torch.stack([c0, c1, c2, c3], dim=2).flatten(1)[:, :columns]
+
+
+def dropout(x: torch.Tensor, drop) -> torch.Tensor:
+    """``elementwise.dropout`` with a mask in memory; ``drop`` has been checked."""
+    T = x.shape[-2] if x.dim() > 1 else 1
+    t = torch.arange(T, device=x.device) if drop.pos is None else drop.pos
+    seqs = x.numel() // max(1, T * x.shape[-1])
+    row = (torch.arange(seqs, device=x.device)[:, None] * drop.seq_len + t).reshape(-1)
+    keep = philox(row, x.shape[-1], drop.site, drop.seed) >= int(drop.p * 2 ** 32)
+    return torch.where(keep.view(x.shape), x * (1.0 / (1.0 - drop.p)), torch.zeros((), dtype=x.dtype, device=x.device))
+
+
 # ----------------------------------------------------------------------------- RoPE caches
 def yarn_inv_freq(head_dim: int, base: float, scale: float = 1.0, orig_maxpos: float = 1024.0,
                   beta_fast: float = 32.0, beta_slow: float = 1.0) -> Tuple[torch.Tensor, int, int]:

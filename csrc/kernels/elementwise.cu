@@ -42,15 +42,72 @@ __device__ __forceinline__ void load8f(const float* __restrict__ p, int c, float
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
+// ============================================================================ dropout
+// Whether an element is kept is a function of its place alone, so no mask is stored: backward, recomputed activations and the ranks of a
+// context-parallel group draw it again.  Philox4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011) with
+// seven rounds, the fewest that pass BigCrush there: counter (column / 4, row, row >> 32, site), key the 64-bit seed, one 32-bit
+// word for each of four columns.  `row` is the global one: sequence * seq_len + position.  An element is kept where its word >= p * 2^32.
+struct Drop {
+  const int64_t* seed;       // one value in device memory, so that a captured launch takes a new one at every replay
+  const int64_t* pos;        // [T] global positions of a sequence's rows, or null: 0 .. T - 1
+  int T;                     // rows of a sequence here
+  long seq_len;              // rows of a whole sequence
+  uint32_t site, threshold;
+  float scale;               // 1 / (1 - p)
+};
+struct DropKey { uint32_t k0, k1; };
+__device__ __forceinline__ DropKey drop_key(const Drop& q) {
+  const uint64_t s = (uint64_t)*q.seed;
+  return DropKey{(uint32_t)s, (uint32_t)(s >> 32)};
+}
+__device__ __forceinline__ uint64_t drop_row(const Drop& q, unsigned row) {
+  const unsigned b = row / (unsigned)q.T, t = row - b * (unsigned)q.T;
+  return (uint64_t)b * (uint64_t)q.seq_len + (uint64_t)(q.pos ? q.pos[t] : (int64_t)t);
+}
+__device__ __forceinline__ uint4 philox7(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, DropKey k) {
+#pragma unroll
+  for (int r = 0; r < 7; ++r) {
+    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k.k0; c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k.k1; c3 = (uint32_t)a;
+    k.k0 += 0x9E3779B9u; k.k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+// The eight columns of vector c of a row: v = v / (1 - p) or 0.  One rounding of the product, and none fused into what follows, as a
+// multiplication of its own has it; a dropped NaN or infinity is gone.
+__device__ __forceinline__ void drop8(const Drop& q, DropKey k, uint64_t row, int c, float (&v)[8]) {
+  const uint4 a = philox7(2u * c, (uint32_t)row, (uint32_t)(row >> 32), q.site, k);
+  const uint4 b = philox7(2u * c + 1u, (uint32_t)row, (uint32_t)(row >> 32), q.site, k);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = w[j] >= q.threshold ? __fmul_rn(v[j], q.scale) : 0.f;
+}
+
+// y = drop(x); its own gradient, too.  Bound by memory: 2 bytes in and 2 out per element.
+__global__ void __launch_bounds__(256)
+dropout_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, unsigned nvec, unsigned total, Drop q) {
+  pdl_release();
+  pdl_wait();
+  const DropKey key = drop_key(q);
+  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+    const unsigned row = i / nvec;
+    float v[8];
+    unpack8(x[i], v);
+    drop8(q, key, drop_row(q, row), (int)(i - row * nvec), v);
+    y[i] = pack8(v);
+  }
+}
+
 // ============================================================================ norm forward
 // One warp per row; d % 8 == 0; MAXV = max 16-byte vectors per lane (d <= 256*MAXV).
-// If `res` != null: x_new = x + res is written to `xout` and normalised.
+// If `res` != null: x_new = x + res is written to `xout` and normalised; DROP: x_new = x + drop(res).
 // LAYER = true -> LayerNorm (mean/var, optional bias); false -> RMSNorm.
-template <bool LAYER, int MAXV>
+template <bool LAYER, int MAXV, bool DROP>
 __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
                                 const float* __restrict__ w, const float* __restrict__ b,
                                 __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
-                                float* __restrict__ stats, int rows, int d, float eps) {
+                                float* __restrict__ stats, int rows, int d, float eps, Drop q) {
   pdl_release();
   pdl_wait();
   const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -70,6 +127,9 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
       if (rr) pr[i] = rr[c];
     }
   }
+  DropKey key{};
+  uint64_t place = 0;
+  if (DROP) { key = drop_key(q); place = drop_row(q, (unsigned)row); }
   float s = 0.f, ss = 0.f;
 #pragma unroll
   for (int i = 0; i < MAXV; ++i) {
@@ -80,8 +140,9 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
       if (rr) {
         float r8[8];
         unpack8(pr[i], r8);
+        if (DROP) drop8(q, key, place, c, r8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r8[j];
+        for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(v[j], r8[j]);
         px[i] = pack8(v);
         ((uint4*)(xout + (size_t)row * d))[c] = px[i];
         unpack8(px[i], v);
@@ -122,12 +183,13 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
 // One warp per row, with dw / db added to shared memory, spent its time in those additions (compare-and-swap loops).
 // Cold L2, one warp per row -> this, us: 32768 x 4096 757 -> 206 (5.2 TB/s); 131072 x 2048 732 -> 367 (5.9); 8192 x 2048
 // 71 -> 36; 8192 x 384 20.5 -> 16.4; layer norm 4096 x 768 20.5 -> 16.3, 4096 x 384 16.4 -> 12.3.
-template <bool LAYER, int G>
+// DROP: the gradient of the dropped branch, drop(dx), goes to `dbranch`.
+template <bool LAYER, int G, bool DROP>
 __global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
 norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy,
                 const __nv_bfloat16* __restrict__ dres, const float* __restrict__ w,
                 const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx,
-                float* __restrict__ dw, float* __restrict__ db, int rows, int d) {
+                float* __restrict__ dw, float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
   pdl_release();
   pdl_wait();
   constexpr int TB = G > 256 ? 512 : 256, NG = TB / G, W = G / 32, R = 4;
@@ -139,6 +201,8 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
 #pragma unroll
   for (int j = 0; j < 8; ++j) { wv[j] = 0.f; aw[j] = 0.f; ab[j] = 0.f; }
   if (on) load8f(w, c, 1.f, wv);
+  DropKey key{};
+  if (DROP) key = drop_key(q);
   int buf = 0;
   for (long base = (long)blockIdx.x * NG * R; base < rows; base += (long)gridDim.x * NG * R, buf ^= 1) {
     const long row0 = base + g * R;
@@ -205,6 +269,10 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
         if (dres) o[j] += r8[j];
       }
       ((uint4*)(dx + (size_t)(row0 + r) * d))[c] = pack8(o);
+      if (DROP) {
+        drop8(q, key, drop_row(q, (unsigned)(row0 + r)), c, o);
+        ((uint4*)(dbranch + (size_t)(row0 + r) * d))[c] = pack8(o);
+      }
     }
   }
   // the groups of a block are added in shared memory, the blocks in global memory.  One group: four columns per addition (one
@@ -899,33 +967,76 @@ static inline int grid_for(size_t work, int block, int per_sm = 8) {
 
 using namespace cpb;
 
-#define NORM_DISPATCH(KERN, LAYER)                                                   \
+// The dropout of a launch; seed == null: none.
+static int make_drop(Drop& q, const int64_t* seed, const int64_t* pos, long rows, int T, long seq_len, long site, double p) {
+  if (seed == nullptr) { q = Drop{}; return CPB_OK; }
+  if (!(p >= 0. && p < 1.)) return set_error(CPB_ERR_ARG, "dropout: p=%g outside [0, 1)", p);
+  if (T <= 0 || rows % T || rows > 0x7fffffffL || seq_len <= 0) return set_error(CPB_ERR_ARG, "dropout: %ld rows in sequences of %d of %ld", rows, T, seq_len);
+  if (site < 0 || site > 0xffffffffL) return set_error(CPB_ERR_ARG, "dropout: site %ld outside 32 bits", site);
+  q = Drop{seed, pos, T, seq_len, (uint32_t)site, (uint32_t)(p * 4294967296.0), (float)(1.0 / (1.0 - p))};
+  return CPB_OK;
+}
+
+// x, y bf16 [rows, d]; see Drop for the rest.
+extern "C" int cpb_dropout(const void* x, void* y, long rows, int d, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site,
+                           double p, cudaStream_t stream) {
+  if (d <= 0 || d % 8) return set_error(CPB_ERR_ARG, "dropout: d=%d must be a multiple of 8", d);
+  if (rows <= 0) return CPB_OK;
+  if (seed == nullptr || ((uintptr_t)x & 15) || ((uintptr_t)y & 15) || rows * (long)(d / 8) >= (1L << 31))
+    return set_error(CPB_ERR_ARG, "dropout: needs a seed, 16-byte aligned rows and less than 2^34 elements");
+  Drop q;
+  const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
+  if (rc != CPB_OK) return rc;
+  const unsigned total = (unsigned)(rows * (d / 8));
+  CPB_CUDA_OK(launch_pdl(dropout_kernel, grid_for(total, 256), 256, 0, stream, (const uint4*)x, (uint4*)y, (unsigned)d / 8, total, q));
+  return check_launch("dropout");
+}
+
+#define NORM_DISPATCH(KERN, LAYER, DROP)                                             \
   do {                                                                               \
     const int nv = (d / 8 + 31) / 32;                                                \
-    if (nv <= 1) kern = KERN<LAYER, 1>;                                              \
-    else if (nv <= 2) kern = KERN<LAYER, 2>;                                         \
-    else if (nv <= 4) kern = KERN<LAYER, 4>;                                         \
-    else if (nv <= 8) kern = KERN<LAYER, 8>;                                         \
-    else if (nv <= 16) kern = KERN<LAYER, 16>;                                       \
+    if (nv <= 1) kern = KERN<LAYER, 1, DROP>;                                        \
+    else if (nv <= 2) kern = KERN<LAYER, 2, DROP>;                                   \
+    else if (nv <= 4) kern = KERN<LAYER, 4, DROP>;                                   \
+    else if (nv <= 8) kern = KERN<LAYER, 8, DROP>;                                   \
+    else if (nv <= 16) kern = KERN<LAYER, 16, DROP>;                                 \
     else return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);              \
   } while (0)
+
+static int norm_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y, float* stats, int rows, int d, float eps,
+                    int layer, const Drop& q, cudaStream_t stream) {
+  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
+  if (rows <= 0) return CPB_OK;
+  const int wpb = 8;
+  decltype(&norm_fwd_kernel<true, 1, false>) kern;
+  if (q.seed != nullptr) {
+    if (layer) NORM_DISPATCH(norm_fwd_kernel, true, true);
+    else NORM_DISPATCH(norm_fwd_kernel, false, true);
+  } else {
+    if (layer) NORM_DISPATCH(norm_fwd_kernel, true, false);
+    else NORM_DISPATCH(norm_fwd_kernel, false, false);
+  }
+  CPB_CUDA_OK(launch_pdl(kern, (rows + wpb - 1) / wpb, wpb * 32, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)res, w, b, (__nv_bfloat16*)xout, (__nv_bfloat16*)y, stats, rows, d, eps, q));
+  return check_launch("norm_fwd");
+}
 
 // x (+res) -> xout (only when res != null), y ; stats [rows,2] (mean, rstd) optional
 extern "C" int cpb_norm_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y,
                             float* stats, int rows, int d, float eps, int layer, cudaStream_t stream) {
-  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
-  if (rows <= 0) return CPB_OK;
-  const int wpb = 8;
-  decltype(&norm_fwd_kernel<true, 1>) kern;
-  if (layer) NORM_DISPATCH(norm_fwd_kernel, true);
-  else NORM_DISPATCH(norm_fwd_kernel, false);
-  CPB_CUDA_OK(launch_pdl(kern, (rows + wpb - 1) / wpb, wpb * 32, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)res, w, b, (__nv_bfloat16*)xout, (__nv_bfloat16*)y, stats, rows, d, eps));
-  return check_launch("norm_fwd");
+  return norm_fwd(x, res, w, b, xout, y, stats, rows, d, eps, layer, Drop{}, stream);
 }
 
-// dw / db are fp32 and accumulated into (+=).
-extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats,
-                            void* dx, float* dw, float* db, int rows, int d, int layer, cudaStream_t stream) {
+// x + drop(res) -> xout, y
+extern "C" int cpb_norm_drop_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y, float* stats, int rows, int d,
+                                 float eps, int layer, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site, double p, cudaStream_t stream) {
+  if (res == nullptr || seed == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs a residual branch and a seed");
+  Drop q;
+  const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
+  return rc != CPB_OK ? rc : norm_fwd(x, res, w, b, xout, y, stats, rows, d, eps, layer, q, stream);
+}
+
+static int norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, float* dw, float* db, int rows,
+                    int d, int layer, void* dbranch, const Drop& q, cudaStream_t stream) {
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
   const int nvec = d / 8;
@@ -934,9 +1045,10 @@ extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, con
   do {                                                                                                                          \
     const int tb = G > 256 ? 512 : 256, per_block = 4 * (tb / G);                                                               \
     const int cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block, blocks = need < cap ? need : cap; \
-    auto kern = layer ? norm_bwd_kernel<true, G> : norm_bwd_kernel<false, G>;                                                   \
+    auto kern = q.seed != nullptr ? (layer ? norm_bwd_kernel<true, G, true> : norm_bwd_kernel<false, G, true>)                  \
+                                  : (layer ? norm_bwd_kernel<true, G, false> : norm_bwd_kernel<false, G, false>);               \
     CPB_CUDA_OK(launch_pdl(kern, blocks, tb, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats,    \
-                                    (__nv_bfloat16*)dx, dw, db, rows, d));                                                       \
+                                    (__nv_bfloat16*)dx, dw, db, rows, d, (__nv_bfloat16*)dbranch, q));                           \
   } while (0)
   if (nvec <= 32) NORM_BWD(32);
   else if (nvec <= 64) NORM_BWD(64);
@@ -945,6 +1057,22 @@ extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, con
   else NORM_BWD(512);
 #undef NORM_BWD
   return check_launch("norm_bwd");
+}
+
+// dw / db are fp32 and accumulated into (+=).
+extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats,
+                            void* dx, float* dw, float* db, int rows, int d, int layer, cudaStream_t stream) {
+  return norm_bwd(x, dy, dres, w, stats, dx, dw, db, rows, d, layer, nullptr, Drop{}, stream);
+}
+
+// as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped
+extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, void* dbranch,
+                                 float* dw, float* db, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site,
+                                 double p, cudaStream_t stream) {
+  if (dbranch == nullptr || seed == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs the branch's gradient and a seed");
+  Drop q;
+  const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
+  return rc != CPB_OK ? rc : norm_bwd(x, dy, dres, w, stats, dx, dw, db, rows, d, layer, dbranch, q, stream);
 }
 
 extern "C" int cpb_swiglu_fwd(const void* gu, void* act, long rows, int F, cudaStream_t stream) {
