@@ -74,7 +74,7 @@ KNOWN_ENV = {
     "CP_RING_SIZE", "CP_HYBRID_GQA",
     # this framework's additions
     "CP_FUSED", "CP_WATCHDOG_S", "CP_NVLS", "CP_GRAD_BUCKET_MB", "CP_DKV_MODE", "CP_SHARD_OPTIM", "CP_AR_CTAS",
-    "CP_GRAPH_POOL_MB",
+    "CP_GRAPH_POOL_MB", "CP_DROPOUT",
     "CP_FUSED_HYBRID_ULYSSES", "CP_LOAD_BALANCE", "CP_INIT_DEVICE", "CP_TEST_LOG_DIR", "CP_NATIVE_PG",
 }
 
@@ -185,6 +185,7 @@ class Config:
     min_lr: float = 6e-5
     weight_decay: float = 0.1
     grad_clip: float = 1.0
+    dropout: float = 0.0                # embedding and both residual branches of a block, in training passes; none on attention weights
     beta1: float = 0.9
     beta2: float = 0.95
     adam_eps: float = 1e-8
@@ -333,6 +334,8 @@ class Config:
             die("CP_CREAM_MODE requires CP_SIZE=1 (bluscriptCP.cpp:717-719)")
         if self.eval_ppl and self.dp_size != 1:
             die("CP_EVAL_PPL requires DP=1")
+        if not 0.0 <= self.dropout < 1.0:
+            die(f"CP_DROPOUT={self.dropout} must be in [0, 1)")
         if self.dkv_mode not in ("route", "pull"):
             die(f"CP_DKV_MODE={self.dkv_mode!r} must be route|red|pull")
         if self.recompute not in ("none", "selective", "full"):
@@ -371,6 +374,7 @@ def _common(env, world_size):
         ring_outer=_flag(env, "CP_RING_OUTER"),
         recompute_k=_flag(env, "CP_RECOMPUTE_K"),
         recompute=_str(env, "CP_RECOMPUTE", "none"),
+        dropout=_float(env, "CP_DROPOUT", 0.0),
         no_grad_allreduce=_flag(env, "CP_NO_GRAD_ALLREDUCE"),
         ring_bf16=_flag(env, "CP_RING_BF16", True),
         save_kv_bf16=_flag(env, "CP_SAVE_KV_BF16", True),

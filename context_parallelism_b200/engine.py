@@ -83,6 +83,7 @@ class TrainEngine:
         if cfg.no_grad_allreduce:
             self.reducer.enabled = False
         self.step_idx = 0
+        self._micro = 0                     # micro-batches since the last update
         self.resume_anchor = -1
         self._pos_dev = {}
         self.last_grad_norm: Optional[torch.Tensor] = None
@@ -125,6 +126,7 @@ class TrainEngine:
 
     def forward_backward(self, tokens, targets, accum: int = 1, last: bool = True) -> torch.Tensor:
         tokens, targets = self._taken(tokens), self._taken(targets)
+        self._next_dropout()
         if self._recordable(targets):
             return self._recorded_micro_batch(tokens, targets, accum)
         idx, tgt, pos = self.shard_batch(tokens, targets)
@@ -139,6 +141,14 @@ class TrainEngine:
         if last:
             self.reducer.finish()
         return loss_sum.detach() / n_local
+
+    def _next_dropout(self) -> None:
+        """A seed of its own for every micro-batch, from what a resumed run knows as well: the configuration's seed, the step, the
+        micro-batch and the data-parallel rank.  The ranks of a context-parallel group drop the same elements."""
+        if self.cfg.dropout > 0:
+            seed = dropout_seed(self.cfg.seed, self.cp.dp_rank, self.step_idx, self._micro)
+            self.model.dropout_seed = torch.full((1,), seed, dtype=torch.int64, device=self.device)
+            self._micro += 1
 
     def _recordable(self, targets) -> bool:
         """One GPU and nothing but this package's own forward and backward pass in the micro-batch."""
@@ -161,6 +171,7 @@ class TrainEngine:
         norm = self.opt.step(lr, self.cfg.grad_clip)
         self.opt.zero_grad()
         self.step_idx += 1
+        self._micro = 0
         self.last_grad_norm = norm
         return norm
 
@@ -208,6 +219,17 @@ class TrainEngine:
         if self.cp.fused is not None:
             self.cp.fused.close()
             self.cp.fused = None
+
+
+def dropout_seed(*parts: int) -> int:
+    """The parts mixed into 64 bits, signed (the steps of splitmix64, Steele, Lea, Flood 2014, once per part)."""
+    mask, h = (1 << 64) - 1, 0
+    for part in parts:
+        h = (h + part + 0x9E3779B97F4A7C15) & mask
+        h = ((h ^ h >> 30) * 0xBF58476D1CE4E5B9) & mask
+        h = ((h ^ h >> 27) * 0x94D049BB133111EB) & mask
+        h ^= h >> 31
+    return h - (1 << 64) if h >> 63 else h
 
 
 class _null:

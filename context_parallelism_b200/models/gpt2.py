@@ -43,13 +43,13 @@ class GPT2Block(nn.Module):
         self.c_fc_w, self.c_fc_b = normal((4 * d, d), 0.02), nn.Parameter(torch.zeros(4 * d))
         self.mlp_proj_w, self.mlp_proj_b = normal((d, 4 * d), resid), nn.Parameter(torch.zeros(d))
 
-    def pre_attention(self, x, pending):
-        h, x = E.layernorm(x, self.ln_1_w, self.ln_1_b, 1e-5, pending)
+    def pre_attention(self, x, pending, drop=None):
+        h, x = E.layernorm(x, self.ln_1_w, self.ln_1_b, 1e-5, pending, None if pending is None else drop)
         return x, G.linear(h, self.c_attn_w, self.c_attn_b)
 
-    def post_attention(self, x, attn_out):
+    def post_attention(self, x, attn_out, drop=None):
         a = G.linear(attn_out, self.attn_proj_w, self.attn_proj_b)
-        h, x = E.layernorm(x, self.ln_2_w, self.ln_2_b, 1e-5, a)
+        h, x = E.layernorm(x, self.ln_2_w, self.ln_2_b, 1e-5, a, drop)
         act = G.linear_gelu(h, self.c_fc_w, self.c_fc_b)
         return x, G.linear(act, self.mlp_proj_w, self.mlp_proj_b)
 
@@ -70,6 +70,8 @@ class GPT2(nn.Module):
         self.lm_head = None if cfg.weight_tying else nn.Parameter(
             _padded_normal(cfg.vocab_size, cfg.vocab_padded, d, gen))
         self.to(device)
+        # what the next training pass drops (one int64 on the device); the engine puts a new one here for every micro-batch
+        self.dropout_seed = torch.tensor([cfg.seed], dtype=torch.int64, device=device) if cfg.dropout > 0 else None
         self.attn = CPAttention(cfg, self.cp)
         self.graphs = graphs.GraphCache(cfg.graph_pool_mb << 20, _WRITTEN)
 
@@ -93,51 +95,58 @@ class GPT2(nn.Module):
 
     def hidden(self, idx_local: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         if torch.is_grad_enabled() or not self.recordable():
-            return self._hidden(idx_local, pos)
+            return self._hidden(idx_local, pos, *self.recorded_inputs())
         return self.graphs.run("hidden", self, lambda i, p: (self._hidden(i, p),), (idx_local, pos), self.wte.device,
                                graphs.model_flops(self.cfg, *idx_local.shape, False))[0]
 
     def recorded_inputs(self) -> tuple:
         """What ``loss_with`` reads beside its tokens, targets and positions and the weights."""
-        return ()
+        return () if self.dropout_seed is None or not (self.training and torch.is_grad_enabled()) else (self.dropout_seed,)
 
     def recordable(self) -> bool:
         """One GPU and the methods of this class (``graphs`` looks at the blocks and the attention)."""
         return self.cp.cp_size == 1 and _WRITTEN.model_holds(self)
 
-    def _hidden(self, idx_local: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+    def _hidden(self, idx_local: torch.Tensor, pos: torch.Tensor, drop_seed: Optional[torch.Tensor] = None) -> torch.Tensor:
         cfg = self.cfg
         x = E.embedding(idx_local, self.wte, pos, self.wpe)
         pending = None
+        # a place in the model is a site; a token's row is its global one, whichever rank holds it
+        drop = None if drop_seed is None else E.Dropout(cfg.dropout, drop_seed, 0, pos.long(), idx_local.shape[1] * self.cp.cp_size)
+        at = (lambda site: ()) if drop is None else (lambda site: (drop._replace(site=site),))
+        if drop is not None:
+            x = E.dropout(x, drop)
         use_ckpt = cfg.recompute in ("selective", "full") and torch.is_grad_enabled()
         full = cfg.recompute == "full" and torch.is_grad_enabled()
         # this package's blocks draw no random numbers, and keeping the generators' states for each part costs the host more than its launches
         draws = use_ckpt and not _WRITTEN.holds(self)
-        for blk in self.blocks:
+        for i, blk in enumerate(self.blocks):
+            before, after = at(2 * i), at(2 * i + 1)
             if full:
-                x, pending = checkpoint(self._block, blk, x, pending, pos, use_reentrant=False, preserve_rng_state=draws)
+                x, pending = checkpoint(self._block, blk, x, pending, pos, before, after, use_reentrant=False, preserve_rng_state=draws)
             elif use_ckpt:
-                x, qkv = checkpoint(blk.pre_attention, x, pending, use_reentrant=False, preserve_rng_state=draws)
+                x, qkv = checkpoint(blk.pre_attention, x, pending, *before, use_reentrant=False, preserve_rng_state=draws)
                 o = self.attn(qkv, pos)
-                x, pending = checkpoint(blk.post_attention, x, o, use_reentrant=False, preserve_rng_state=draws)
+                x, pending = checkpoint(blk.post_attention, x, o, *after, use_reentrant=False, preserve_rng_state=draws)
             else:
-                x, qkv = blk.pre_attention(x, pending)
+                x, qkv = blk.pre_attention(x, pending, *before)
                 o = self.attn(qkv, pos)
-                x, pending = blk.post_attention(x, o)
-        h, _ = E.layernorm(x, self.ln_f_w, self.ln_f_b, 1e-5, pending)
+                x, pending = blk.post_attention(x, o, *after)
+        h, _ = E.layernorm(x, self.ln_f_w, self.ln_f_b, 1e-5, pending, *at(2 * len(self.blocks)))
         return h
 
-    def _block(self, blk, x, pending, pos):
+    def _block(self, blk, x, pending, pos, before=(), after=()):
         """One whole block; ``CP_RECOMPUTE=full`` re-runs it (attention and its communication included) in backward."""
-        x, qkv = blk.pre_attention(x, pending)
+        x, qkv = blk.pre_attention(x, pending, *before)
         o = self.attn(qkv, pos)
-        return blk.post_attention(x, o)
+        return blk.post_attention(x, o, *after)
 
     def head_weight(self) -> torch.Tensor:
         return self.wte if self.lm_head is None else self.lm_head
 
-    def loss_with(self, idx_local, targets_local, pos, grad_scale: float) -> torch.Tensor:
-        return xent.linear_cross_entropy(self._hidden(idx_local, pos), self.head_weight(), targets_local, grad_scale, self.cfg.vocab_size)
+    def loss_with(self, idx_local, targets_local, pos, *seed_and_scale) -> torch.Tensor:
+        *seed, grad_scale = seed_and_scale
+        return xent.linear_cross_entropy(self._hidden(idx_local, pos, *seed), self.head_weight(), targets_local, grad_scale, self.cfg.vocab_size)
 
     def loss_sum(self, idx_local, targets_local, pos, grad_scale: float = 1.0) -> torch.Tensor:
         h = self.hidden(idx_local, pos)

@@ -55,17 +55,17 @@ class LlamaBlock(nn.Module):
 
     # The two halves are separate functions so activation recomputation can wrap each of them while the
     # attention core (by far the most expensive part) is never recomputed.
-    def pre_attention(self, x, pending, cache, pos):
+    def pre_attention(self, x, pending, cache, pos, drop=None):
         cfg = self.cfg
-        h, x = E.rmsnorm(x, self.attn_norm, cfg.rms_eps, pending)
+        h, x = E.rmsnorm(x, self.attn_norm, cfg.rms_eps, pending, None if pending is None else drop)
         qkv = G.linear(h, self.wqkv)
         qkv = E.qk_norm_rope(qkv, self.q_gamma, self.k_gamma, cache, pos, cfg.n_head, cfg.n_kv_head, cfg.head_dim, cfg.qk_eps)
         return x, qkv
 
-    def post_attention(self, x, attn_out):
+    def post_attention(self, x, attn_out, drop=None):
         cfg = self.cfg
         a = G.linear(attn_out, self.wo)
-        h, x = E.rmsnorm(x, self.mlp_norm, cfg.rms_eps, a)
+        h, x = E.rmsnorm(x, self.mlp_norm, cfg.rms_eps, a, drop)
         act = G.linear_swiglu(h, self.gate_up)
         return x, G.linear(act, self.down)
 
@@ -91,6 +91,8 @@ class Llama(nn.Module):
         self.attn = CPAttention(cfg, self.cp)
         self.rope_cache = R.build_rope_cache(cfg.T, cfg.head_dim, cfg.rope_theta, device, cfg.yarn)
         self.rope_pos_override: Optional[torch.Tensor] = None
+        # what the next training pass drops (one int64 on the device); the engine puts a new one here for every micro-batch
+        self.dropout_seed = torch.tensor([cfg.seed], dtype=torch.int64, device=device) if cfg.dropout > 0 else None
         self.graphs = graphs.GraphCache(cfg.graph_pool_mb << 20, _WRITTEN)
 
     # ------------------------------------------------------------------ RoPE cache control
@@ -134,42 +136,52 @@ class Llama(nn.Module):
 
     def recorded_inputs(self) -> tuple:
         """What ``loss_with`` reads beside its tokens, targets and positions and the weights: these are swapped between calls."""
-        return (self.rope_cache,) if self.rope_pos_override is None else (self.rope_cache, self.rope_pos_override)
+        rope = (self.rope_cache,) if self.rope_pos_override is None else (self.rope_cache, self.rope_pos_override)
+        if self.dropout_seed is None or not (self.training and torch.is_grad_enabled()):
+            return rope
+        none = self.rope_cache.new_empty(0)                  # floating point, so no positions
+        return (*rope, self.dropout_seed) if len(rope) == 2 else (*rope, none, self.dropout_seed)
 
     def recordable(self) -> bool:
         """One GPU and the methods of this class (``graphs`` looks at the blocks and the attention)."""
         return self.cp.cp_size == 1 and _WRITTEN.model_holds(self)
 
     def _hidden(self, idx_local: torch.Tensor, pos: torch.Tensor, rope_cache: torch.Tensor,
-                rope_pos: Optional[torch.Tensor] = None) -> torch.Tensor:
+                rope_pos: Optional[torch.Tensor] = None, drop_seed: Optional[torch.Tensor] = None) -> torch.Tensor:
         cfg = self.cfg
         x = E.embedding(idx_local, self.wte)
         pending = None
-        rpos = pos if rope_pos is None else rope_pos
+        rpos = pos if rope_pos is None or rope_pos.dtype.is_floating_point else rope_pos
+        # a place in the model is a site; a token's row is its global one, whichever rank holds it
+        drop = None if drop_seed is None else E.Dropout(cfg.dropout, drop_seed, 0, pos.long(), idx_local.shape[1] * self.cp.cp_size)
+        at = (lambda site: ()) if drop is None else (lambda site: (drop._replace(site=site),))
+        if drop is not None:
+            x = E.dropout(x, drop)
         use_ckpt = cfg.recompute in ("selective", "full") and torch.is_grad_enabled()
         full = cfg.recompute == "full" and torch.is_grad_enabled()
         # this package's blocks draw no random numbers, and keeping the generators' states for each part costs the host more than its launches
         draws = use_ckpt and not _WRITTEN.holds(self)
-        for blk in self.blocks:
+        for i, blk in enumerate(self.blocks):
+            before, after = at(2 * i), at(2 * i + 1)
             if full:
                 # full activation recompute: only the block's input survives the forward pass; backward re-runs the
                 # whole block, context-parallel attention (and its communication) included, on every rank alike
-                x, pending = checkpoint(self._block, blk, x, pending, rope_cache, rpos, pos, use_reentrant=False, preserve_rng_state=draws)
+                x, pending = checkpoint(self._block, blk, x, pending, rope_cache, rpos, pos, before, after, use_reentrant=False, preserve_rng_state=draws)
             elif use_ckpt:
-                x, qkv = checkpoint(blk.pre_attention, x, pending, rope_cache, rpos, use_reentrant=False, preserve_rng_state=draws)
+                x, qkv = checkpoint(blk.pre_attention, x, pending, rope_cache, rpos, *before, use_reentrant=False, preserve_rng_state=draws)
                 o = self.attn(qkv, pos)
-                x, pending = checkpoint(blk.post_attention, x, o, use_reentrant=False, preserve_rng_state=draws)
+                x, pending = checkpoint(blk.post_attention, x, o, *after, use_reentrant=False, preserve_rng_state=draws)
             else:
-                x, qkv = blk.pre_attention(x, pending, rope_cache, rpos)
+                x, qkv = blk.pre_attention(x, pending, rope_cache, rpos, *before)
                 o = self.attn(qkv, pos)
-                x, pending = blk.post_attention(x, o)
-        h, _ = E.rmsnorm(x, self.norm_f, cfg.rms_eps, pending)
+                x, pending = blk.post_attention(x, o, *after)
+        h, _ = E.rmsnorm(x, self.norm_f, cfg.rms_eps, pending, *at(2 * len(self.blocks)))
         return h
 
-    def _block(self, blk, x, pending, rope_cache, rpos, pos):
-        x, qkv = blk.pre_attention(x, pending, rope_cache, rpos)
+    def _block(self, blk, x, pending, rope_cache, rpos, pos, before=(), after=()):
+        x, qkv = blk.pre_attention(x, pending, rope_cache, rpos, *before)
         o = self.attn(qkv, pos)
-        return blk.post_attention(x, o)
+        return blk.post_attention(x, o, *after)
 
     def head_weight(self) -> torch.Tensor:
         return self.wte if self.lm_head is None else self.lm_head

@@ -105,3 +105,67 @@ def test_a_norm_without_a_branch_has_nothing_to_drop():
         E.rmsnorm(x, None, 1e-5, None, E.Dropout(0.1, _seed()))
     with pytest.raises(AssertionError):
         E.rmsnorm(x, None, 1e-5, x[:, :1], E.Dropout(0.1, _seed()))
+
+
+def _engine(family="llama", recompute="none", dropout=0.2, **kw):
+    from context_parallelism_b200.config import Config
+    from context_parallelism_b200.engine import TrainEngine
+    cfg = Config.from_env(family, 1, env={"CP_DROPOUT": str(dropout)}).replace(**{**dict(
+        n_embd=64, n_layer=2, n_head=2, n_kv_head=2, head_dim=32, ffn_hidden=128, vocab_size=100, T=16, B=2, dtype="fp32", recompute=recompute,
+        checkpointing=False), **kw})
+    return TrainEngine(cfg, torch.device("cpu"))
+
+
+def _batch(eng, seed=0):
+    t = torch.randint(0, eng.cfg.vocab_size, (eng.cfg.B, eng.cfg.T + 1), generator=torch.Generator().manual_seed(seed))
+    return t[:, :-1].contiguous(), t[:, 1:].contiguous()
+
+
+@pytest.mark.parametrize("family", ["llama", "gpt2"])
+def test_models(family):
+    engines = [_engine(family, r) for r in ("none", "selective", "full")]
+    for step in range(2):
+        losses = [[float(e.forward_backward(*_batch(e, i), accum=2, last=i == 1)) for i in range(2)] for e in engines]
+        assert losses[0] == losses[1] == losses[2]
+        for e in engines[1:]:
+            assert torch.equal(e.flat.grad, engines[0].flat.grad)
+        for e in engines:
+            e.optimizer_step()
+    # the same tokens, another micro-batch, other elements; without gradients nothing is dropped
+    a, b = engines[0], _engine(family, dropout=0.0)
+    assert float(a.forward_backward(*_batch(a))) != float(a.forward_backward(*_batch(a)))
+    b.flat.master.copy_(a.flat.master)
+    assert float(a.eval_loss(*_batch(a))) == float(b.eval_loss(*_batch(b)))
+    assert float(a.forward_backward(*_batch(a))) != float(b.forward_backward(*_batch(b)))
+    idx, tgt, pos = a.shard_batch(*_batch(a))
+    a.model.eval()
+    assert torch.equal(a.model.hidden(idx, pos), b.model.hidden(idx, pos))
+
+
+def test_every_site_drops_on_its_own():
+    from context_parallelism_b200.ops import elementwise
+    eng, seen = _engine(), []
+    kept = elementwise.ref.dropout
+    try:
+        elementwise.ref.dropout = lambda x, drop: seen.append((drop.site, int(drop.seed), drop.seq_len, drop.pos.tolist())) or kept(x, drop)
+        eng.forward_backward(*_batch(eng))
+        eng.forward_backward(*_batch(eng))
+    finally:
+        elementwise.ref.dropout = kept
+    pos = list(range(eng.cfg.T))
+    seeds = [seen[0][1], seen[5][1]]
+    assert seeds[0] != seeds[1] and seen == [(s, seed, eng.cfg.T, pos) for seed in seeds for s in (0, 1, 2, 3, 4)]
+
+
+def test_seeds():
+    from context_parallelism_b200.engine import dropout_seed
+    seeds = {dropout_seed(1234, r, s, m) for r in range(4) for s in range(16) for m in range(8)}
+    assert len(seeds) == 4 * 16 * 8 and all(-2 ** 63 <= s < 2 ** 63 for s in seeds)
+
+
+def test_configuration():
+    from context_parallelism_b200.config import Config
+    assert Config.from_env("gpt2", 1, env={}).dropout == 0.0
+    for bad in (-0.1, 1.0, float("nan")):
+        with pytest.raises(ValueError):
+            Config.from_env("llama", 1, env={}).replace(dropout=bad).validate()
