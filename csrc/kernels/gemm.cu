@@ -134,8 +134,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();      // 0: even CTA (issues the MMAs), 1: odd CTA
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  const int num_tiles = p.num_m_tiles * p.num_n_blocks;
-  const int num_items = num_tiles * p.splits;   // item = split * num_tiles + tile: items of one K range run together
+  int num_m_tiles = p.num_m_tiles, num_k_blocks = p.num_k_blocks, k_per_split = p.k_per_split;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -156,6 +155,24 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   if (p.splits == 1) pdl_release();
   pdl_wait();
   const uint32_t tmem_base = *tmem_slot;
+  if (p.live.count != nullptr) {
+    const int n = max(0, min(__ldg(p.live.count) - p.live.before, p.live.of_k ? p.K : p.M));
+    if (p.live.of_k) {
+      num_k_blocks = (n + GEMM_BK - 1) / GEMM_BK;
+      k_per_split = max(1, (num_k_blocks + p.splits - 1) / p.splits);
+      if (n == 0 && p.splits == 1 && p.epi == EPI_F32_ACC) num_m_tiles = 0;      // nothing to add
+    } else {
+      num_m_tiles = (n + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
+    }
+  }
+  const int num_tiles = num_m_tiles * p.num_n_blocks;
+  const int num_items = num_tiles * p.splits;   // item = split * num_tiles + tile: items of one K range run together
+  // the K blocks of a split; one that has none left takes the first block behind the operands, which TMA fills with zeros
+  const auto k_range = [&](int split, int& kb0, int& kb1) {
+    kb0 = split * k_per_split;
+    kb1 = min(num_k_blocks, kb0 + k_per_split);
+    if (kb0 >= kb1) { kb0 = p.num_k_blocks; kb1 = kb0 + 1; }
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -166,10 +183,11 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (int item = pair; item < num_items; item += num_pairs) {
         const int split = item / num_tiles;
         int mt, nb;
-        pair_tile_coords(item - split * num_tiles, p.num_m_tiles, p.num_n_blocks, p.band, mt, nb);
+        pair_tile_coords(item - split * num_tiles, num_m_tiles, p.num_n_blocks, p.band, mt, nb);
         const int m0 = mt * (2 * GEMM_BM) + (int)rank * GEMM_BM;      // this CTA's rows
-        const int kb1 = min(p.num_k_blocks, (split + 1) * p.k_per_split);
-        for (int kb = split * p.k_per_split; kb < kb1; ++kb) {
+        int kb0, kb1;
+        k_range(split, kb0, kb1);
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag, p.status, 110)) break;
           uint8_t* sa = smem + stage * L::STAGE_BYTES;
           uint8_t* sb = sa + L::A_BYTES;
@@ -226,7 +244,8 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * L::ACC_COLS;
         const int split = item / num_tiles;
-        const int kb0 = split * p.k_per_split, kb1 = min(p.num_k_blocks, kb0 + p.k_per_split);
+        int kb0, kb1;
+        k_range(split, kb0, kb1);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[stage], phase, abort_flag, p.status, 211))) { alive = false; break; }
           tc_fence_after();
@@ -259,7 +278,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const int acc = L::ACCS == 2 ? it & 1 : 0;
       const uint32_t acc_phase = (L::ACCS == 2 ? it >> 1 : it) & 1;
       int mt, nb;
-      pair_tile_coords(item % num_tiles, p.num_m_tiles, p.num_n_blocks, p.band, mt, nb);
+      pair_tile_coords(item % num_tiles, num_m_tiles, p.num_n_blocks, p.band, mt, nb);
       const int row0 = mt * (2 * GEMM_BM) + (int)rank * GEMM_BM + quarter * 32;
       const HeadRow head = head_row(p, row0 + lane);
       bool ok = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, p.status, 310);
@@ -464,9 +483,9 @@ using namespace cpb;
 // epi: see EPI_* above.  For EPI_BF16_SWIGLU B is the fused [2F, K] weight, N = F output features.
 // splits > 1 (accumulating and bf16 epilogues, see cpb_gemm_plan): K is split that often; partials is a 16-byte aligned workspace of
 // splits - 1 (bf16: splits) matrices of M x N floats, and a second launch adds them to C (bf16: sums them, adds the bias and rounds once).
-extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, const float* bias,
-                             int M, int N, int K, int lda, int ldb, int ldc, int ld_aux,
-                             int a_mn, int b_mn, int epi, float* partials, int splits, int* status, cudaStream_t stream) {
+static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const float* bias,
+                     int M, int N, int K, int lda, int ldb, int ldc, int ld_aux,
+                     int a_mn, int b_mn, int epi, float* partials, int splits, const Live& live, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0) return set_error(CPB_ERR_ARG, "gemm: empty problem %dx%dx%d", M, N, K);
   // the contiguous dimension of every operand and every row stride must be a multiple of 8 elements (16 bytes)
   if ((N % 8) || (lda % 8) || (ldb % 8)) return set_error(CPB_ERR_ARG, "gemm: N,lda,ldb must be multiples of 8 (got N=%d lda=%d ldb=%d)", N, lda, ldb);
@@ -495,7 +514,7 @@ extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, c
   p.band = tile_band(N, K);
   const int per_tile = epi == EPI_BF16_SWIGLU ? bn / 2 : bn;
   p.num_n_blocks = (N + per_tile - 1) / per_tile;
-  p.has_aux = aux != nullptr; p.bias = bias; p.status = status;
+  p.has_aux = aux != nullptr; p.bias = bias; p.status = status; p.live = live;
   const bool sum16 = splits > 1 && epi == EPI_BF16;      // every split goes to the workspace, the sum kernel writes C
   if (sum16) { p.epi = EPI_F32; p.bias = nullptr; }
 
@@ -535,20 +554,20 @@ extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, c
   return check_launch("gemm_add_partials");
 }
 
-// Cross entropy of the language-model head, logits = x w^T (x [M,K], w [N,K], both K-major).  out == null or fp32 (grad == 0): per row and
-// 256-wide tile (max, sum of exponentials) to stats [ceil(N / 256)][M] and the target's logit; out, if given, gets the logits as well.
-// grad == 1: out (bf16) = (softmax - onehot) * grad_scale from row_coef (cpb_xent_rows).  out: [M,N], row stride ldc.
-//
-// The gradient pass computes the logits again, 2 K operations for each, where storing them in fp32 moves 4 bytes for the GEMM and 4
-// more for the kernel that turns them into dlogits; beyond a K of about a thousand storing them is cheaper (cpb_xent_dlogits).
-extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int64_t* targets, float* stats, float* target_logit,
-                             const float* row_coef, int M, int N, int K, int ldx, int ldw, int ldc, int n_valid, int grad, float grad_scale,
-                             int* status, cudaStream_t stream) {
+extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, const float* bias,
+                             int M, int N, int K, int lda, int ldb, int ldc, int ld_aux,
+                             int a_mn, int b_mn, int epi, float* partials, int splits, int* status, cudaStream_t stream) {
+  return gemm_bf16(A, B, C, aux, bias, M, N, K, lda, ldb, ldc, ld_aux, a_mn, b_mn, epi, partials, splits, Live{}, status, stream);
+}
+
+static int gemm_head(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
+                     const Live& live, int* status, cudaStream_t stream) {
+  const int n_valid = head.n_valid;
   if (M <= 0 || N <= 0 || K <= 0) return set_error(CPB_ERR_ARG, "gemm_head: empty problem %dx%dx%d", M, N, K);
   if ((N % 8) || (K % 8) || (ldx % 8) || (ldw % 8) || (out && (ldc % 8)))
     return set_error(CPB_ERR_ARG, "gemm_head: N,K,ldx,ldw,ldc must be multiples of 8 (got N=%d K=%d ldx=%d ldw=%d ldc=%d)", N, K, ldx, ldw, ldc);
   if (n_valid <= 0 || n_valid > N) return set_error(CPB_ERR_ARG, "gemm_head: n_valid=%d outside 1..%d", n_valid, N);
-  if (grad ? (out == nullptr || row_coef == nullptr) : (stats == nullptr || target_logit == nullptr)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
+  if (grad ? (out == nullptr || head.row_coef == nullptr) : (head.stats == nullptr || head.target_logit == nullptr)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
   GemmParams p{};
   p.M = M; p.N = N; p.K = K; p.epi = grad ? EPI_HEAD_GRAD : out ? EPI_HEAD_STORE : EPI_HEAD_STATS;
   p.num_m_tiles = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
@@ -556,7 +575,8 @@ extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int6
   p.num_k_blocks = p.k_per_split = (K + GEMM_BK - 1) / GEMM_BK;
   p.splits = 1;
   p.band = tile_band(N, K);
-  p.head = HeadParams{targets, (float2*)stats, target_logit, (const float2*)row_coef, n_valid, grad_scale};
+  p.head = head;
+  p.live = live;
   p.status = status;
   CUtensorMap tm[4];
   int rc;
@@ -572,6 +592,35 @@ extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int6
   tm[3] = tm[2];
   return launch_pair<256, false, false>(tm, p, stream);
 }
+
+// Cross entropy of the language-model head, logits = x w^T (x [M,K], w [N,K], both K-major).  out == null or fp32 (grad == 0): per row and
+// 256-wide tile (max, sum of exponentials) to stats [ceil(N / 256)][M] and the target's logit; out, if given, gets the logits as well.
+// grad == 1: out (bf16) = (softmax - onehot) * grad_scale from row_coef (cpb_xent_rows).  out: [M,N], row stride ldc.
+//
+// The gradient pass computes the logits again, 2 K operations for each, where storing them in fp32 moves 4 bytes for the GEMM and 4
+// more for the kernel that turns them into dlogits; beyond a K of about a thousand storing them is cheaper (cpb_xent_dlogits).
+extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int64_t* targets, float* stats, float* target_logit,
+                             const float* row_coef, int M, int N, int K, int ldx, int ldw, int ldc, int n_valid, int grad, float grad_scale,
+                             int* status, cudaStream_t stream) {
+  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, HeadParams{targets, (float2*)stats, target_logit, (const float2*)row_coef, n_valid, grad_scale, nullptr},
+                   Live{}, status, stream);
+}
+
+// The same two for objectives.cu, with rows counted on the device.
+namespace cpb {
+int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t stream) {
+  return gemm_bf16(g.A, g.B, g.C, nullptr, nullptr, g.M, g.N, g.K, g.lda, g.ldb, g.ldc, 0, g.a_mn, g.b_mn, g.epi, g.partials, g.splits, live, status, stream);
+}
+int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
+                   const Live& live, int* status, cudaStream_t stream) {
+  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, status, stream);
+}
+int gemm_splits(int M, int N, int K, int epi) {
+  int bn = 256, splits = 1;
+  if (M > 0 && N > 0 && K > 0) plan_tiles(M, N, K, epi, 0, 0, bn, splits);
+  return splits;
+}
+}  // namespace cpb
 
 // The plan of a GEMM of this shape and epilogue: tile width << 16 | how often K is split (at least 1).  For a split the caller brings the
 // workspace, splits - 1 matrices of M x N floats for the accumulating epilogue, splits for the bf16 one.

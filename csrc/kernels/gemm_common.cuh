@@ -32,9 +32,19 @@ struct HeadParams {
   const int64_t* targets;    // [M]; a row whose target is outside [0, n_valid) has neither loss nor gradient
   float2* stats;             // [tiles along N][M] (max, sum of exp(x - max))
   float* target_logit;       // [M], written where the target is in range
-  const float2* row_coef;    // [M] (max, grad_scale / sum), (max, 0) for ignored rows
+  const float2* row_coef;    // [M] (max, grad_scale / sum), (max, 0) for ignored rows; with row_scale (max, 1 / sum)
   int n_valid;               // columns from here on are padding
   float grad_scale;
+  const float* row_scale;    // [M] or null: a scale for each row in the place of grad_scale; 0: no gradient, whatever the row holds
+};
+
+// How much of a GEMM's M or K is there, as a number in device memory: the rows that the kernels of objectives.cu have gathered, of which a
+// launch takes those behind the first `before`.  Tiles of rows behind them are not computed.  For K, what the operands hold behind them up
+// to the next multiple of 64 has to be zero.
+struct Live {
+  const int* count;          // null: all of M and K
+  int before;
+  int of_k;                  // 0: rows of A and C, 1: K
 };
 
 struct GemmParams {
@@ -48,6 +58,7 @@ struct GemmParams {
   int band;            // pair-rows per band of the tile order (1 = rows of tiles, columns fastest)
   int has_aux;
   const float* bias;
+  Live live;
   HeadParams head;
   int* status;
 };
@@ -132,13 +143,21 @@ __device__ __forceinline__ float pick64(const float (&f)[64], int at) {
 struct HeadRow {
   int target;                // column, or negative
   float2 coef;
+  float scale;               // of the target's one
+  bool off;                  // a row of zeros
 };
 __device__ __forceinline__ HeadRow head_row(const GemmParams& p, int row) {
-  HeadRow h{-1, {0.f, 0.f}};
+  HeadRow h{-1, {0.f, 0.f}, p.head.grad_scale, false};
   if (p.epi >= EPI_HEAD_STATS && row < p.M) {
     const int64_t t = __ldg(p.head.targets + row);
     h.target = t >= 0 && t < p.head.n_valid ? (int)t : -1;
     if (p.epi == EPI_HEAD_GRAD) h.coef = __ldg(p.head.row_coef + row);
+    if (p.head.row_scale != nullptr) {
+      h.scale = __ldg(p.head.row_scale + row);
+      h.coef.y *= h.scale;
+      h.off = h.scale == 0.f;
+      if (h.off) h.target = -1;
+    }
   }
   return h;
 }
@@ -214,7 +233,11 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
       }
       if (hit) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) f[j] = j == at ? f[j] - p.head.grad_scale : f[j];
+        for (int j = 0; j < 64; ++j) f[j] = j == at ? f[j] - h.scale : f[j];
+      }
+      if (h.off) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) f[j] = 0.f;
       }
       uint32_t v[32];
       pack_row(f, v);
@@ -326,5 +349,18 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
     }
   }
 }
+
+// gemm.cu, for objectives.cu
+struct GemmLive {
+  const void *A, *B;
+  void* C;
+  int M, N, K, lda, ldb, ldc, a_mn, b_mn, epi;
+  float* partials;           // workspace of gemm_splits(M, N, K, epi) > 1: as many matrices of M x N floats (accumulating: one less)
+  int splits;
+};
+int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t stream);
+int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
+                   const Live& live, int* status, cudaStream_t stream);
+int gemm_splits(int M, int N, int K, int epi);
 
 }  // namespace cpb

@@ -1,0 +1,522 @@
+// Fine-tuning objectives over the language-model head: log-probabilities of tokens, the clipped policy loss with a KL term, the paired
+// log-ratio loss.  All three are functions of logp_i = z_it - log sum_j exp(z_ij), z = x w^T, of the tokens that count, and have the gradient
+// dz_ij = h_i (1[j = t] - p_ij) with one number h_i = dloss / dlogp_i per token, dx = dz w, dw = dz^T x.
+//
+// Of a fine-tuning batch only the answers' tokens count, a third to two thirds of it.  So the counted rows are gathered first, in their order
+// (rows_count, rows_gather), and the GEMMs behind read from device memory how many there are (Live in gemm_common.cuh): masked tokens cost
+// nothing, whatever they hold, and the host does not wait for the number.  Then as for the cross entropy (xent.cu): the head's GEMM leaves
+// (max, sum of exponentials) per row and tile of 256 columns, rows_finish makes logp and h of them, and for the gradient a second GEMM
+// computes the logits again or, for wide hidden states, reads the fp32 ones that the first has stored.  Everything per token is
+// computed in 64 bits: e^d - d - 1 of two nearly equal log-probabilities and the sums over long answers need it, and there are few tokens.
+// Every sum has a fixed order: a call repeats bit for bit.
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "host_utils.h"
+
+namespace cpb {
+
+struct Rows {                // the gathered rows, kept from the forward pass to the backward pass
+  int* live;                 // [0] how many, [1] a ticket
+  int* from;                 // [N] gathered row -> row
+  int* place;                // [N] row -> gathered row, or -1
+  int64_t* targets;          // [N] gathered
+  float2* norm;              // [N] gathered: (max, 1 / sum of exponentials)
+  float* h;                  // [N] gathered: dloss / dlogp, written by the policy loss
+  __nv_bfloat16* x;          // [N, d] gathered, zero from the last row to the next multiple of 64
+  float* logits;             // [N, V] gathered, or null
+};
+
+__device__ __forceinline__ bool row_counts(const int64_t* targets, const float* weights, int row, int n_valid) {
+  const int64_t t = targets[row];
+  return t >= 0 && t < n_valid && (weights == nullptr || weights[row] != 0.f);
+}
+
+// Counted rows of every 32; the rows that do not count have a log-probability of 0.
+__global__ void __launch_bounds__(256)
+rows_count_kernel(const int64_t* __restrict__ targets, const float* __restrict__ weights, int* __restrict__ counts, float* __restrict__ logp,
+                  int* __restrict__ live, int N, int n_valid, int* status) {
+  pdl_release();
+  pdl_wait();
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  bool on = false;
+  if (row < N) {
+    on = row_counts(targets, weights, row, n_valid);
+    if (targets[row] >= n_valid) report(status, ST_BAD_INDEX, 1300, (int)targets[row]);
+    logp[row] = 0.f;
+  }
+  const unsigned mask = __ballot_sync(0xffffffffu, on);
+  if ((threadIdx.x & 31) == 0 && row < N) counts[row >> 5] = __popc(mask);
+  if (row == 0) live[1] = 0;
+}
+
+// Gathers 32 rows per block: x[b, t] has strides sb and st.  Bound by memory, 2 d bytes in and out per row.
+__global__ void __launch_bounds__(256)
+rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T, int d, const int64_t* __restrict__ targets,
+                   const float* __restrict__ weights, const int* __restrict__ counts, Rows r, int N, int n_valid) {
+  pdl_release();
+  pdl_wait();
+  __shared__ int part[8], s_base, s_n, s_from[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x;
+  int before = 0;
+  for (int i = threadIdx.x; i < group; i += 256) before += counts[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) part[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    int base = 0;
+    for (int i = 0; i < 8; ++i) base += part[i];
+    const int row = group * 32 + lane;
+    const bool on = row < N && row_counts(targets, weights, row, n_valid);
+    const unsigned mask = __ballot_sync(0xffffffffu, on);
+    const int rank = __popc(mask & ((1u << lane) - 1u));
+    if (on) {
+      s_from[rank] = row;
+      r.from[base + rank] = row;
+      r.targets[base + rank] = targets[row];
+    }
+    if (row < N) r.place[row] = on ? base + rank : -1;
+    if (lane == 0) { s_base = base; s_n = __popc(mask); }
+    if (lane == 0 && group == (int)gridDim.x - 1) r.live[0] = base + __popc(mask);
+  }
+  __syncthreads();
+  const int nvec = d >> 3;
+  for (int i = warp; i < s_n; i += 8) {
+    const int row = s_from[i], b = row / T;
+    const uint4* src = (const uint4*)(x + b * sb + (row - b * T) * st);
+    uint4* dst = (uint4*)(r.x + (size_t)(s_base + i) * d);
+    for (int c = lane; c < nvec; c += 128) {
+      uint4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) v[k] = src[c + 32 * k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) dst[c + 32 * k] = v[k];
+    }
+  }
+  if (group == (int)gridDim.x - 1) {                               // K of the weight gradient is taken 64 rows at a time
+    const int total = s_base + s_n, end = min(N, (total + 63) & ~63);
+    for (int i = total + warp; i < end; i += 8)
+      for (int c = lane; c < nvec; c += 32) ((uint4*)(r.x + (size_t)i * d))[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+struct Policy {
+  const float *old_logp, *advantages, *weights, *ref_logp;         // [N] by row; weights and ref_logp may be null
+  double low, high, kl;                                            // the ratio is clipped to [low, high]
+  double* part;                                                    // [blocks][4]
+  float* sums;                                                     // [5] out: loss, then sums of weight x (surrogate, KL, clipped, 1)
+};
+
+// Between the two passes of the head's GEMM: logp and (max, 1 / sum) of 32 gathered rows per block, and for a policy loss its terms and h.
+// A warp takes every eighth tile (the lanes' pairs are adjacent in memory), warp 0 adds the eight parts, always in the same order.
+constexpr int RF_WARPS = 8;
+template <bool POLICY>
+__global__ void __launch_bounds__(RF_WARPS * 32)
+rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logit, Rows r, float* __restrict__ logp, int before, int rows,
+                   int tiles, Policy q, int blocks_before, int blocks) {
+  pdl_release();
+  pdl_wait();
+  __shared__ float2 part[RF_WARPS][32];
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;                          // in this launch
+  const int at = before + row;                                     // gathered
+  const bool on = row < rows && at < r.live[0];
+  float m = -INFINITY, s = 0.f;
+  // a part without a finite maximum contributes its sum as it is: zero, or NaN
+  const auto add = [&](float2 v) {
+    const float mn = fmaxf(m, v.x);
+    s = (m == -INFINITY ? s : s * __expf(m - mn)) + (v.x == -INFINITY ? v.y : v.y * __expf(v.x - mn));
+    m = mn;
+  };
+  if (on) {
+    int t = warp;
+    for (; t + 3 * RF_WARPS < tiles; t += 4 * RF_WARPS) {
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = stats[(size_t)(t + k * RF_WARPS) * rows + row];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) add(v[k]);
+    }
+    for (; t < tiles; t += RF_WARPS) add(stats[(size_t)t * rows + row]);
+  }
+  part[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (warp == 0) {
+    for (int k = 1; k < RF_WARPS; ++k) add(part[k][lane]);
+    double sur = 0., kl = 0., cut = 0., wt = 0.;
+    if (on) {
+      const double lp = (double)target_logit[row] - (double)m - log((double)s);
+      r.norm[at] = make_float2(m, 1.f / s);
+      const int from = r.from[at];
+      logp[from] = (float)lp;
+      if (POLICY) {
+        const double a = q.advantages[from], ratio = exp(lp - (double)q.old_logp[from]);
+        wt = q.weights ? (double)q.weights[from] : 1.;
+        const bool c = (a > 0. && ratio > q.high) || (a < 0. && ratio < q.low);
+        // an advantage of nothing has no surrogate, however far the ratio is
+        sur = a == 0. ? 0. : -a * (c ? (a > 0. ? q.high : q.low) : ratio);
+        double h = a == 0. || c ? 0. : sur;                        // d(-a r) / dlogp = -a r
+        if (q.ref_logp) {
+          const double delta = (double)q.ref_logp[from] - lp, e = expm1(delta);
+          kl = e - delta;
+          h -= q.kl * e;
+        }
+        r.h[at] = (float)(wt * h);
+        sur *= wt; kl *= wt; cut = c ? wt : 0.;
+      }
+    }
+    if (POLICY) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        sur += __shfl_xor_sync(0xffffffffu, sur, o); kl += __shfl_xor_sync(0xffffffffu, kl, o);
+        cut += __shfl_xor_sync(0xffffffffu, cut, o); wt += __shfl_xor_sync(0xffffffffu, wt, o);
+      }
+      if (lane == 0) {
+        double* out = q.part + 4 * (size_t)(blocks_before + blockIdx.x);
+        out[0] = sur; out[1] = kl; out[2] = cut; out[3] = wt;
+        __threadfence();
+        s_last = atomicAdd(r.live + 1, 1) == blocks - 1;           // of all launches of the call
+      }
+    }
+  }
+  if (!POLICY) return;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  // the last block adds all parts: thread by thread, then the threads in order
+  __shared__ double total[RF_WARPS][4];
+  double v[4] = {0., 0., 0., 0.};
+  for (int i = threadIdx.x; i < blocks; i += RF_WARPS * 32)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __ldcg(q.part + 4 * (size_t)i + k);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (lane == 0)
+    for (int k = 0; k < 4; ++k) total[warp][k] = v[k];
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < RF_WARPS; ++w)
+    for (int k = 0; k < 4; ++k) total[0][k] += total[w][k];
+  q.sums[0] = (float)(q.ref_logp ? total[0][0] + q.kl * total[0][1] : total[0][0]);
+  for (int k = 0; k < 4; ++k) q.sums[1 + k] = (float)total[0][k];
+}
+
+// Sums of 256 threads in a fixed order; thread 0 has the result.
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int i = 1; i < 8; ++i) v += scratch[i];
+  return v;
+}
+
+// sums[b][s] = sum over the s-th part of sequence b of logp - ref, of the tokens that count.
+__global__ void __launch_bounds__(256)
+sequence_sums_kernel(const float* __restrict__ logp, const float* __restrict__ ref, const int64_t* __restrict__ targets, double* __restrict__ sums,
+                     int T, int part, int n_valid) {
+  pdl_release();
+  pdl_wait();
+  __shared__ double scratch[8];
+  const int b = blockIdx.y, t0 = blockIdx.x * part, t1 = min(T, t0 + part);
+  double v = 0.;
+  for (int t = t0 + threadIdx.x; t < t1; t += 256) {
+    const size_t i = (size_t)b * T + t;
+    if (targets[i] >= 0 && targets[i] < n_valid) v += (double)logp[i] - (double)ref[i];
+  }
+  v = block_sum(v, scratch);
+  if (threadIdx.x == 0) sums[(size_t)b * gridDim.x + blockIdx.x] = v;
+}
+
+// Pairs (i, pairs + i): the loss, the log-ratio of every sequence and dloss / dlogp of its tokens.
+__global__ void __launch_bounds__(256)
+preference_kernel(const double* __restrict__ sums, int parts, int pairs, const float* __restrict__ weights, double beta, double smoothing,
+                  float* __restrict__ loss, float* __restrict__ ratios, float* __restrict__ h) {
+  pdl_release();
+  pdl_wait();
+  __shared__ double scratch[8];
+  double l = 0.;
+  for (int i = threadIdx.x; i < pairs; i += 256) {
+    double c = 0., r = 0.;
+    for (int k = 0; k < parts; ++k) {
+      c += sums[(size_t)i * parts + k];
+      r += sums[(size_t)(pairs + i) * parts + k];
+    }
+    ratios[i] = (float)c; ratios[pairs + i] = (float)r;
+    const double wt = weights ? (double)weights[i] : 1.;
+    double g = 0.;
+    if (wt != 0.) {
+      // softplus(-z) = max(-z, 0) + log1p(e^-|z|); its derivative -sigma(-z)
+      const double z = beta * (c - r), e = exp(-fabs(z)), small = log1p(e), pos = 1. / (1. + e), neg = e / (1. + e);
+      const double up = z > 0. ? pos : z <= 0. ? neg : z, down = z > 0. ? neg : z <= 0. ? pos : z;      // sigma(z), sigma(-z); NaN stays
+      l += wt * ((1. - smoothing) * (fmax(-z, 0.) + small) + smoothing * (fmax(z, 0.) + small));
+      g = wt * beta * (smoothing * up - (1. - smoothing) * down);
+    }
+    h[i] = (float)g; h[pairs + i] = (float)-g;
+  }
+  l = block_sum(l, scratch);
+  if (threadIdx.x == 0) *loss = (float)l;
+}
+
+// scale = -g dloss/dlogp of the gathered rows, 0 behind the last: what xent.cu calls grad_scale, row by row.  h is by gathered row (each ==
+// 0) or by row / each.
+__global__ void __launch_bounds__(256)
+rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, float* __restrict__ scale, int N) {
+  pdl_release();
+  pdl_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= N) return;
+  float v = 0.f;
+  if (i < r.live[0]) {
+    v = -(each == 0 ? h[i] : h[r.from[i] / each]);
+    if (g) v *= *g;
+  }
+  scale[i] = v;
+}
+
+// dlogits of gathered rows from stored logits.  Bound by memory: 4 bytes in and 2 out per logit; four 16-byte loads per thread before the
+// first use.  Rows behind the last one are zero up to the next multiple of 64, see Live.
+constexpr int RD_COLS = 256 * 16;
+__global__ void __launch_bounds__(256)
+rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V) {
+  pdl_release();
+  pdl_wait();
+  const int row = blockIdx.y, at = before + row, live = r.live[0];
+  if (at >= ((live + 63) & ~63)) return;
+  const float s = scale[at];
+  const bool on = s != 0.f;                                        // a row of gradient 0 is zero, whatever its logits are
+  float top = 0.f, inv = 0.f;
+  int64_t tgt = -1;
+  if (on) { top = r.norm[at].x; inv = r.norm[at].y * s; tgt = r.targets[at]; }
+  const int c0 = blockIdx.x * RD_COLS + 4 * threadIdx.x;
+  const float4* x = (const float4*)(r.logits + (size_t)at * V);
+  float4 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on && c0 + 1024 * k < V) v[k] = x[(c0 + 1024 * k) >> 2];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = c0 + 1024 * k;
+    if (c >= V) break;
+    float p[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      p[e] = on && c + e < n_valid ? __expf(p[e] - top) * inv : 0.f;
+      if (tgt == c + e) p[e] -= s;
+    }
+    *(uint2*)(dlogits + (size_t)row * V + c) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+  }
+}
+
+// dx of every row: the gathered row's, or 0.
+__global__ void __launch_bounds__(256)
+rows_scatter_kernel(const __nv_bfloat16* __restrict__ in, const int* __restrict__ place, __nv_bfloat16* __restrict__ out, int N, int d) {
+  pdl_release();
+  pdl_wait();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, nvec = d >> 3;
+  if (row >= N) return;
+  const int at = place[row];
+  const uint4* src = (const uint4*)(in + (size_t)max(at, 0) * d);
+  uint4* dst = (uint4*)(out + (size_t)row * d);
+  for (int c = lane; c < nvec; c += 128) {
+    uint4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (at >= 0 && c + 32 * k < nvec) v[k] = src[c + 32 * k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) dst[c + 32 * k] = v[k];
+  }
+}
+
+// fp32 gradient of the weights, added up over chunks of rows, as bf16
+__global__ void __launch_bounds__(256)
+weight_cast_kernel(const float4* __restrict__ in, uint4* __restrict__ out, size_t n8) {
+  pdl_release();
+  pdl_wait();
+  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < n8; i += (size_t)gridDim.x * 256) {
+    const float4 a = in[2 * i], b = in[2 * i + 1];
+    out[i] = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
+  }
+}
+
+// ------------------------------------------------------------------ layout of the buffers
+static size_t take(size_t& at, size_t bytes) {
+  const size_t here = at;
+  at = (at + bytes + 255) & ~(size_t)255;
+  return here;
+}
+// `base` may be null: the size alone
+static Rows rows_layout(char* base, long N, int d, long V, int store, size_t& bytes) {
+  size_t at = 0;
+  Rows r;
+  r.live = (int*)(base + take(at, 256));
+  r.from = (int*)(base + take(at, N * 4));
+  r.place = (int*)(base + take(at, N * 4));
+  r.targets = (int64_t*)(base + take(at, N * 8));
+  r.norm = (float2*)(base + take(at, N * 8));
+  r.h = (float*)(base + take(at, N * 4));
+  r.x = (__nv_bfloat16*)(base + take(at, (size_t)N * d * 2));
+  r.logits = store ? (float*)(base + take(at, (size_t)N * V * 4)) : nullptr;
+  bytes = at;
+  return r;
+}
+struct FwdScratch { int* counts; float2* stats; float* target_logit; double* part; };
+static FwdScratch fwd_layout(char* base, long N, long V, int chunk, size_t& bytes) {
+  size_t at = 0;
+  const long rows = N < chunk ? N : chunk, tiles = (V + 255) / 256;
+  FwdScratch s;
+  s.counts = (int*)(base + take(at, (N + 31) / 32 * 4));
+  s.stats = (float2*)(base + take(at, (size_t)tiles * rows * 8));
+  s.target_logit = (float*)(base + take(at, rows * 4));
+  s.part = (double*)(base + take(at, ((N + 31) / 32 + N / chunk + 1) * 32));
+  bytes = at;
+  return s;
+}
+// Where dw goes: nowhere, added to an fp32 buffer, or as bf16 (through an fp32 buffer where there are several chunks of rows).
+enum : int { DW_NONE = 0, DW_ADD = 1, DW_BF16 = 2 };
+struct BwdScratch { float* scale; __nv_bfloat16 *dlogits, *dx; float *dw, *partials; size_t partial_bytes; };
+static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int dw, int want_dx, size_t& bytes) {
+  size_t at = 0;
+  const long rows = N < chunk ? N : chunk;
+  const bool one = N <= chunk;
+  BwdScratch s;
+  s.scale = (float*)(base + take(at, N * 4));
+  s.dlogits = (__nv_bfloat16*)(base + take(at, (size_t)rows * V * 2));
+  s.dx = (__nv_bfloat16*)(base + take(at, want_dx ? (size_t)N * d * 2 : 0));
+  s.dw = (float*)(base + take(at, dw == DW_BF16 && !one ? (size_t)V * d * 4 : 0));
+  size_t most = 0;
+  for (long r0 = 0; r0 < N; r0 += chunk) {                         // the last chunk has a plan of its own
+    const long n = N - r0 < chunk ? N - r0 : chunk;
+    if (r0 > 0 && n == chunk) continue;
+    if (want_dx) {
+      const int k = gemm_splits((int)n, d, (int)V, EPI_BF16);
+      if (k > 1 && (size_t)k * n * d > most) most = (size_t)k * n * d;
+    }
+    if (dw != DW_NONE) {
+      const int epi = dw == DW_BF16 && one ? EPI_BF16 : EPI_F32_ACC, k = gemm_splits((int)V, d, (int)n, epi);
+      const size_t m = (size_t)(epi == EPI_BF16 ? k : k - 1) * V * d;
+      if (k > 1 && m > most) most = m;
+    }
+  }
+  s.partials = (float*)(base + take(at, most * 4));
+  bytes = at;
+  return s;
+}
+
+}  // namespace cpb
+
+using namespace cpb;
+
+// Bytes of the buffers of an objective over N rows of width d and V columns: kept between the passes, of the forward pass, of the backward pass.
+extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int store, int dw, int want_dx, int64_t* bytes) {
+  if (N <= 0 || d <= 0 || V <= 0 || chunk <= 0 || chunk % 256) return set_error(CPB_ERR_ARG, "objective: %d rows of %d, %d columns, chunks of %d", N, d, V, chunk);
+  size_t a, b, c;
+  rows_layout(nullptr, N, d, V, store, a);
+  fwd_layout(nullptr, N, V, chunk, b);
+  bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, c);
+  bytes[0] = (int64_t)a; bytes[1] = (int64_t)b; bytes[2] = (int64_t)c;
+  return CPB_OK;
+}
+
+static int objective_args(int N, int d, int V, int n_valid, int ldw, int chunk) {
+  if (N <= 0 || d <= 0 || V <= 0) return set_error(CPB_ERR_ARG, "objective: empty problem, %d rows of %d, %d columns", N, d, V);
+  if ((d % 8) || (V % 8) || (ldw % 8)) return set_error(CPB_ERR_ARG, "objective: widths and row strides must be multiples of 8 (got d=%d V=%d ldw=%d)", d, V, ldw);
+  if (n_valid <= 0 || n_valid > V) return set_error(CPB_ERR_ARG, "objective: n_valid=%d outside 1..%d", n_valid, V);
+  if (chunk <= 0 || chunk % 256 || chunk > 65280) return set_error(CPB_ERR_ARG, "objective: chunks of %d rows", chunk);
+  return CPB_OK;
+}
+
+// x bf16 [B, T, d] (strides sb, st, rows 16-byte aligned), w bf16 [V, d], targets [B, T]; a row counts where 0 <= target < n_valid and, with
+// `weights`, its weight is not 0.  logp [B, T].  With `advantages`, the policy loss: old_logp, advantages, weights, ref_logp [B, T] (the
+// last two may be null) and sums [5], see Policy.  kept and scratch: cpb_objective_plan.
+extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, int d, const void* w, int ldw, int V, int n_valid, const int64_t* targets,
+                                 const float* old_logp, const float* advantages, const float* weights, const float* ref_logp, double low, double high,
+                                 double kl, float* logp, float* sums, void* kept, int store, void* scratch, int chunk, int* status, cudaStream_t stream) {
+  int rc = objective_args(N, d, V, n_valid, ldw, chunk);
+  if (rc != CPB_OK) return rc;
+  if (T <= 0 || N % T || (sb % 8) || (st % 8) || ((uintptr_t)x & 15)) return set_error(CPB_ERR_ARG, "objective: hidden states need 16-byte aligned rows");
+  size_t bytes;
+  const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
+  const FwdScratch s = fwd_layout((char*)scratch, N, V, chunk, bytes);
+  const int groups = (N + 31) / 32, tiles = (V + 255) / 256;
+  CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
+  CPB_CUDA_OK(launch_pdl(rows_gather_kernel, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, r, N, n_valid));
+  int blocks = 0;
+  for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
+  const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, sums};
+  for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
+    const int n = N - r0 < chunk ? N - r0 : chunk;
+    const HeadParams head{r.targets + r0, s.stats, s.target_logit, nullptr, n_valid, 0.f, nullptr};
+    if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, store ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, 0, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+    auto kern = advantages ? rows_finish_kernel<true> : rows_finish_kernel<false>;
+    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, s.stats, s.target_logit, r, logp, r0, n, tiles, q, done, blocks));
+    done += (n + 31) / 32;
+  }
+  return check_launch("objective_fwd");
+}
+
+// sums fp64 [2 pairs][parts] of logp - ref over the counted tokens of every sequence of T tokens, part by part.
+extern "C" int cpb_sequence_sums(const float* logp, const float* ref, const int64_t* targets, double* sums, int seqs, int T, int parts, int n_valid,
+                                 cudaStream_t stream) {
+  if (seqs <= 0 || T <= 0 || parts <= 0 || seqs > 65535) return set_error(CPB_ERR_ARG, "sequence_sums: %d sequences of %d in %d parts", seqs, T, parts);
+  CPB_CUDA_OK(launch_pdl(sequence_sums_kernel, dim3(parts, seqs), 256, 0, stream, logp, ref, targets, sums, T, (T + parts - 1) / parts, n_valid));
+  return check_launch("sequence_sums");
+}
+
+// loss [1], ratios [2 pairs] and h [2 pairs] from the sums; weights [pairs] or null.
+extern "C" int cpb_preference(const double* sums, int parts, int pairs, const float* weights, double beta, double smoothing, float* loss, float* ratios,
+                              float* h, cudaStream_t stream) {
+  if (pairs <= 0 || parts <= 0) return set_error(CPB_ERR_ARG, "preference: %d pairs in %d parts", pairs, parts);
+  CPB_CUDA_OK(launch_pdl(preference_kernel, 1, 256, 0, stream, sums, parts, pairs, weights, beta, smoothing, loss, ratios, h));
+  return check_launch("preference");
+}
+
+// Gradients: h is dloss / dlogp of row i at h[i / each] (h null: the policy loss's, as the forward pass has left it), g a factor in device
+// memory or null.  dx bf16 [N, d] or null.  dw: DW_ADD fp32 [V, d], added to; DW_BF16 bf16 [V, d].
+extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, int n_valid, const float* h, int each, const float* g, void* dx, void* dw,
+                                 int dw_kind, const void* kept, int store, void* scratch, int chunk, int* status, cudaStream_t stream) {
+  int rc = objective_args(N, d, V, n_valid, ldw, chunk);
+  if (rc != CPB_OK) return rc;
+  if ((h != nullptr && each <= 0) || dw_kind < DW_NONE || dw_kind > DW_BF16 || (dw_kind != DW_NONE && dw == nullptr))
+    return set_error(CPB_ERR_ARG, "objective: gradients of %d rows each, weights' gradient of kind %d", each, dw_kind);
+  size_t bytes;
+  const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
+  const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, dw_kind, dx != nullptr, bytes);
+  const bool one = N <= chunk;
+  CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h ? h : (const float*)r.h, h ? each : 0, g, s.scale, N));
+  for (int r0 = 0; r0 < N; r0 += chunk) {
+    const int n = N - r0 < chunk ? N - r0 : chunk;
+    if (store) {
+      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, s.dlogits, n_valid, V));
+    } else {
+      const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0};
+      if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+    }
+    if (dx != nullptr) {
+      GemmLive m{s.dlogits, w, s.dx + (size_t)r0 * d, n, d, V, V, ldw, d, 0, 1, EPI_BF16, s.partials, gemm_splits(n, d, V, EPI_BF16)};
+      if ((rc = gemm_live(m, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+    }
+    if (dw_kind != DW_NONE) {
+      const bool direct = dw_kind == DW_BF16 && one;
+      const int epi = direct ? EPI_BF16 : dw_kind == DW_BF16 && r0 == 0 ? EPI_F32 : EPI_F32_ACC;
+      GemmLive m{s.dlogits, r.x + (size_t)r0 * d, dw_kind == DW_BF16 && !one ? (void*)s.dw : dw, V, d, n, V, d, d, 1, 1, epi, s.partials,
+                 epi == EPI_F32 ? 1 : gemm_splits(V, d, n, epi)};
+      if ((rc = gemm_live(m, Live{r.live, r0, 1}, status, stream)) != CPB_OK) return rc;
+    }
+  }
+  if (dw_kind == DW_BF16 && !one) {
+    const size_t n8 = (size_t)V * d / 8, blocks = (n8 + 255) / 256, cap = (size_t)sm_count() * 8;
+    CPB_CUDA_OK(launch_pdl(weight_cast_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, (const float4*)s.dw, (uint4*)dw, n8));
+  }
+  if (dx != nullptr)
+    CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (N + 7) / 8, 256, 0, stream, s.dx, r.place, (__nv_bfloat16*)dx, N, d));
+  return check_launch("objective_bwd");
+}
