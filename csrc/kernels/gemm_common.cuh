@@ -27,6 +27,8 @@ enum : int {
   EPI_HEAD_GRAD = 7,   // C(bf16) = (softmax - onehot(target)) * grad_scale from the rows' (max, grad_scale / sum)
 };
 
+constexpr float LOG2E = 1.4426950408889634f;
+
 // Cross entropy in the epilogue of the head's GEMM (xent.cu has the kernel between the two passes).
 struct HeadParams {
   const int64_t* targets;    // [M]; a row whose target is outside [0, n_valid) has neither loss nor gradient
@@ -36,6 +38,7 @@ struct HeadParams {
   int n_valid;               // columns from here on are padding
   float grad_scale;
   const float* row_scale;    // [M] or null: a scale for each row in the place of grad_scale; 0: no gradient, whatever the row holds
+  float l2e = LOG2E;         // what a difference of two logits is multiplied with before 2^x is taken
 };
 
 // How much of a GEMM's M or K is there, as a number in device memory: the rows that the kernels of objectives.cu have gathered, of which a
@@ -129,8 +132,6 @@ __device__ __forceinline__ void pack_row(const float (&f)[64], uint32_t (&v)[32]
   for (int j = 0; j < 32; ++j) v[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
 }
 
-__device__ __forceinline__ float head_exp(float x, float m) { return ex2f((x - m) * 1.4426950408889634f); }
-
 // f[at] without dynamic register indexing (at in [0, 64))
 __device__ __forceinline__ float pick64(const float (&f)[64], int at) {
   float r = 0.f;
@@ -204,10 +205,10 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
         for (int j = 8; j < 64; j += 8) mx[q] = fmax3(mx[q], f[j + q], f[j + q + 4]);
       }
       const float mt = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-      if (mt > m) { s = m == -INFINITY ? s : s * head_exp(m, mt); m = mt; }
+      if (mt > m) { s = m == -INFINITY ? s : s * ex2f((m - mt) * p.head.l2e); m = mt; }
       // a row of nothing but -inf so far adds nothing; NaN gets into the sum, whatever the maximum says
       const float ref = m == -INFINITY ? 0.f : m;
-      const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(1.4426950408889634f, 1.4426950408889634f);
+      const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
       uint64_t acc[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {
@@ -219,7 +220,7 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
       unpack_f32x2(add_f32x2(acc[0], acc[1]), a, b);
       s += a + b;
     } else {
-      const uint64_t nm = pack_f32x2(-h.coef.x, -h.coef.x), l2e = pack_f32x2(1.4426950408889634f, 1.4426950408889634f);
+      const uint64_t nm = pack_f32x2(-h.coef.x, -h.coef.x), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
       const uint64_t inv = pack_f32x2(h.coef.y, h.coef.y);
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {

@@ -113,7 +113,7 @@ constexpr int RF_WARPS = 8;
 template <bool POLICY>
 __global__ void __launch_bounds__(RF_WARPS * 32)
 rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logit, Rows r, float* __restrict__ logp, int before, int rows,
-                   int tiles, Policy q, int blocks_before, int blocks) {
+                   int tiles, double logits, Policy q, int blocks_before, int blocks) {
   pdl_release();
   pdl_wait();
   __shared__ float2 part[RF_WARPS][32];
@@ -123,10 +123,11 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
   const int at = before + row;                                     // gathered
   const bool on = row < rows && at < r.live[0];
   float m = -INFINITY, s = 0.f;
+  const float l2e = (float)(logits * 1.4426950408889634);
   // a part without a finite maximum contributes its sum as it is: zero, or NaN
   const auto add = [&](float2 v) {
     const float mn = fmaxf(m, v.x);
-    s = (m == -INFINITY ? s : s * __expf(m - mn)) + (v.x == -INFINITY ? v.y : v.y * __expf(v.x - mn));
+    s = (m == -INFINITY ? s : s * ex2f((m - mn) * l2e)) + (v.x == -INFINITY ? v.y : v.y * ex2f((v.x - mn) * l2e));
     m = mn;
   };
   if (on) {
@@ -146,7 +147,7 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
     for (int k = 1; k < RF_WARPS; ++k) add(part[k][lane]);
     double sur = 0., kl = 0., cut = 0., wt = 0.;
     if (on) {
-      const double lp = (double)target_logit[row] - (double)m - log((double)s);
+      const double lp = logits * ((double)target_logit[row] - (double)m) - log((double)s);
       r.norm[at] = make_float2(m, 1.f / s);
       const int from = r.from[at];
       logp[from] = (float)lp;
@@ -282,7 +283,7 @@ rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __
 // first use.  Rows behind the last one are zero up to the next multiple of 64, see Live.
 constexpr int RD_COLS = 256 * 16;
 __global__ void __launch_bounds__(256)
-rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V) {
+rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V, float l2e) {
   pdl_release();
   pdl_wait();
   const int row = blockIdx.y, at = before + row, live = r.live[0];
@@ -307,7 +308,7 @@ rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, __nv_bf
     float p[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      p[e] = on && c + e < n_valid ? __expf(p[e] - top) * inv : 0.f;
+      p[e] = on && c + e < n_valid ? ex2f((p[e] - top) * l2e) * inv : 0.f;
       if (tgt == c + e) p[e] -= s;
     }
     *(uint2*)(dlogits + (size_t)row * V + c) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
@@ -346,6 +347,13 @@ weight_cast_kernel(const float4* __restrict__ in, uint4* __restrict__ out, size_
     out[i] = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
   }
 }
+
+// The tensor core cuts off what an accumulator has no bits for after every 16 of K, so a logit comes out too small in size: half a last place a
+// step, for a sum that grows evenly K 2^-30 of it.  Measured at logits above 8 (spread 4, 50304 and 128256 columns), relative: K 384
+// -3.4e-7, 768 -7.0e-7, 2048 -1.97e-6, 4096 -4.05e-6; this factor takes it back.  A sum that has its size early is off by
+// up to twice that, one that gets it late by next to nothing, so it is nowhere further off with the factor than without.  A single logp hardly
+// shows it, target and normaliser being off alike; sums over an answer do.
+static double logit_scale(int d) { return 1. + (double)d / 1073741824.; }
 
 // ------------------------------------------------------------------ layout of the buffers
 static size_t take(size_t& at, size_t bytes) {
@@ -451,13 +459,14 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   CPB_CUDA_OK(launch_pdl(rows_gather_kernel, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, r, N, n_valid));
   int blocks = 0;
   for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
+  const double logits = logit_scale(d);
   const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, sums};
   for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
-    const HeadParams head{r.targets + r0, s.stats, s.target_logit, nullptr, n_valid, 0.f, nullptr};
+    const HeadParams head{r.targets + r0, s.stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, (float)(logits * 1.4426950408889634)};
     if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, store ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, 0, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
     auto kern = advantages ? rows_finish_kernel<true> : rows_finish_kernel<false>;
-    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, s.stats, s.target_logit, r, logp, r0, n, tiles, q, done, blocks));
+    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, s.stats, s.target_logit, r, logp, r0, n, tiles, logits, q, done, blocks));
     done += (n + 31) / 32;
   }
   return check_launch("objective_fwd");
@@ -491,13 +500,14 @@ extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, in
   const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
   const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, dw_kind, dx != nullptr, bytes);
   const bool one = N <= chunk;
+  const float l2e = (float)(logit_scale(d) * 1.4426950408889634);
   CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h ? h : (const float*)r.h, h ? each : 0, g, s.scale, N));
   for (int r0 = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
     if (store) {
-      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, s.dlogits, n_valid, V));
+      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, s.dlogits, n_valid, V, l2e));
     } else {
-      const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0};
+      const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0, l2e};
       if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
     }
     if (dx != nullptr) {
