@@ -23,10 +23,13 @@ from torch.autograd.function import once_differentiable
 
 from .. import _native as nv
 from .gemm import EPI_BF16, EPI_F32_ACC, acc_splits
-from .xent import RECOMPUTE_WIDTH
 
 CHUNK_BYTES = 2 << 30            # of bf16 dlogits, the rows that go through the gradient's products at a time
-KEEP_BYTES = 16 << 30            # of fp32 logits, kept from the forward to the backward pass for hidden states wider than RECOMPUTE_WIDTH
+KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward to the backward pass
+# Width of the hidden states from which on that is faster than to compute them again.  token_logprobs and its gradient, us, kept and
+# computed again: 4608 x 50304, width 256 567 and 560, 384 664 and 711, 520 1047 and 1153, 768 1001 and 1159, 1024 1245 and 1286; 300 x 50304,
+# 768 199 and 234; 4608 x 8192, 384 199 and 230; 4608 x 128256, 2048 5936 and 7338.
+KEEP_WIDTH = 320
 PART = 4096                      # tokens of a sequence that one block adds up
 
 
@@ -80,10 +83,10 @@ def _plan(N: int, d: int, V: int, chunk: int, store: bool, dw: int, want_dx: boo
 
 @functools.lru_cache(maxsize=4096)
 def _backward_launches(N: int, d: int, V: int, chunk: int, dw: int, want_dx: bool) -> int:
-    n = 1 + want_dx + (dw == 2 and N > chunk)
+    n = 1 + (dw == 2 and N > chunk)
     for r0 in range(0, N, chunk):
         rows = min(chunk, N - r0)
-        n += 1 + (1 + (acc_splits(rows, d, V, EPI_BF16) > 1) if want_dx else 0)
+        n += 1 + 2 * want_dx
         if dw:
             epi = EPI_BF16 if dw == 2 and N <= chunk else EPI_F32_ACC
             n += 1 + (acc_splits(V, d, rows, epi) > 1 and not (dw == 2 and N > chunk and r0 == 0))
@@ -106,7 +109,7 @@ class _Head:
         self.shape, self.w, self.n_valid, self.grad = x.shape, w, n_valid, grad
         self.N, self.d, self.V = targets.numel(), x.shape[-1], w.shape[0]
         self.chunk = _chunk(self.V)
-        self.store = grad and self.d > RECOMPUTE_WIDTH and 4 * self.N * self.V <= KEEP_BYTES
+        self.store = grad and self.d >= KEEP_WIDTH and 2 * self.N * self.V <= KEEP_BYTES
 
 
 def _rows16(t):

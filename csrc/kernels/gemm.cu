@@ -134,7 +134,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();      // 0: even CTA (issues the MMAs), 1: odd CTA
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-  int num_m_tiles = p.num_m_tiles, num_k_blocks = p.num_k_blocks, k_per_split = p.k_per_split;
+  int num_m_tiles = p.num_m_tiles, num_k_blocks = p.num_k_blocks, k_per_split = p.k_per_split, splits = p.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -163,10 +163,14 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (n == 0 && p.splits == 1 && p.epi == EPI_F32_ACC) num_m_tiles = 0;      // nothing to add
     } else {
       num_m_tiles = (n + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
+      if (p.live.splits != nullptr) {
+        splits = max(1, min(__ldg(p.live.splits), p.splits));
+        k_per_split = (num_k_blocks + splits - 1) / splits;
+      }
     }
   }
   const int num_tiles = num_m_tiles * p.num_n_blocks;
-  const int num_items = num_tiles * p.splits;   // item = split * num_tiles + tile: items of one K range run together
+  const int num_items = num_tiles * splits;     // item = split * num_tiles + tile: items of one K range run together
   // the K blocks of a split; one that has none left takes the first block behind the operands, which TMA fills with zeros
   const auto k_range = [&](int split, int& kb0, int& kb1) {
     kb0 = split * k_per_split;
@@ -294,7 +298,8 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           else mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
         }
       };
-      if (p.epi >= EPI_HEAD_STATS) head_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
+      if (p.epi == EPI_HEAD_KEEP) head_keep_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
+      else if (p.epi >= EPI_HEAD_STATS) head_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
       else gemm_epilogue<BN>(p, &tmC, &tmX, ws, t_row, row0, nb, lane, item / num_tiles, release);
     }
     ws.drain();
@@ -567,9 +572,10 @@ static int gemm_head(const void* x, const void* w, void* out, int M, int N, int 
   if ((N % 8) || (K % 8) || (ldx % 8) || (ldw % 8) || (out && (ldc % 8)))
     return set_error(CPB_ERR_ARG, "gemm_head: N,K,ldx,ldw,ldc must be multiples of 8 (got N=%d K=%d ldx=%d ldw=%d ldc=%d)", N, K, ldx, ldw, ldc);
   if (n_valid <= 0 || n_valid > N) return set_error(CPB_ERR_ARG, "gemm_head: n_valid=%d outside 1..%d", n_valid, N);
-  if (grad ? (out == nullptr || head.row_coef == nullptr) : (head.stats == nullptr || head.target_logit == nullptr)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
+  if (grad == 2 && out == nullptr) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
+  if (grad == 1 ? (out == nullptr || head.row_coef == nullptr) : (head.stats == nullptr || head.target_logit == nullptr)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
   GemmParams p{};
-  p.M = M; p.N = N; p.K = K; p.epi = grad ? EPI_HEAD_GRAD : out ? EPI_HEAD_STORE : EPI_HEAD_STATS;
+  p.M = M; p.N = N; p.K = K; p.epi = grad == 2 ? EPI_HEAD_KEEP : grad ? EPI_HEAD_GRAD : out ? EPI_HEAD_STORE : EPI_HEAD_STATS;
   p.num_m_tiles = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
   p.num_n_blocks = (N + 255) / 256;
   p.num_k_blocks = p.k_per_split = (K + GEMM_BK - 1) / GEMM_BK;
@@ -614,6 +620,29 @@ int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t str
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream) {
   return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, status, stream);
+}
+int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const Live& live, int* status,
+                    cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) || (K % 8) || (ldw % 8) || most < 2) return set_error(CPB_ERR_ARG, "gemm_live_parts: %dx%dx%d in %d", M, N, K, most);
+  GemmParams p{};
+  p.M = M; p.N = N; p.K = K; p.epi = EPI_F32;
+  p.num_m_tiles = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
+  p.num_n_blocks = (N + bn - 1) / bn;
+  p.num_k_blocks = (K + GEMM_BK - 1) / GEMM_BK;
+  p.splits = most;
+  p.k_per_split = (p.num_k_blocks + most - 1) / most;
+  p.band = tile_band(N, K);
+  p.status = status;
+  p.live = live;
+  CUtensorMap tm[4];
+  int rc;
+  if ((rc = kmajor_tmap(&tm[0], A, M, K, K, GEMM_BM)) != CPB_OK) return rc;
+  if ((rc = mnmajor_tmap(&tm[1], w, N, K, ldw)) != CPB_OK) return rc;
+  uint64_t dims[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)most}, strides[3] = {0, (uint64_t)N * 4, (uint64_t)M * N * 4};
+  uint32_t box[3] = {32, 32, 1};
+  if ((rc = encode_tmap(&tm[3], parts, 4, 3, dims, strides, box, 1)) != CPB_OK) return rc;
+  tm[2] = tm[3];
+  return bn == 256 ? launch_pair<256, false, true>(tm, p, stream) : bn == 192 ? launch_pair<192, false, true>(tm, p, stream) : launch_pair<128, false, true>(tm, p, stream);
 }
 int gemm_splits(int M, int N, int K, int epi) {
   int bn = 256, splits = 1;

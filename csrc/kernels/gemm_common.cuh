@@ -25,6 +25,7 @@ enum : int {
   EPI_HEAD_STATS = 5,  // language-model head: (max, sum of exponentials) of the tile's columns per row, no C
   EPI_HEAD_STORE = 6,  // both: EPI_HEAD_STATS, and C(f32) = acc
   EPI_HEAD_GRAD = 7,   // C(bf16) = (softmax - onehot(target)) * grad_scale from the rows' (max, grad_scale / sum)
+  EPI_HEAD_KEEP = 8,   // EPI_HEAD_STATS, and C(f16) = acc - the tile's maximum of the row
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -48,6 +49,7 @@ struct Live {
   const int* count;          // null: all of M and K
   int before;
   int of_k;                  // 0: rows of A and C, 1: K
+  const int* splits;         // or null: into how many ranges K is split, at most GemmParams::splits
 };
 
 struct GemmParams {
@@ -161,6 +163,74 @@ __device__ __forceinline__ HeadRow head_row(const GemmParams& p, int row) {
     }
   }
   return h;
+}
+
+// EPI_HEAD_KEEP: what the backward pass needs of the logits, in 16 bits.  f16 of the distance to the tile's maximum is off by 2^-12 of the
+// distance, so the likely tokens, which are near the maximum, come out of it more exactly than the bf16 that their gradient is rounded to
+// in the end.  The accumulator is read twice, for the maximum and for the rest; the sum of exponentials is that of the fp32 values.
+template <int BN, class Release>
+__device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int nb,
+                                                   int lane, const HeadRow& h, Release release) {
+  const int row = row0 + lane;
+  const bool live = row0 < p.M;
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < BN; c += 64) {
+    const int col = nb * BN + c;
+    float f[64];
+    tmem_ld32(t_row + c, *(uint32_t(*)[32])&f[0]);
+    tmem_ld32(t_row + c + 32, *(uint32_t(*)[32])&f[32]);
+    tmem_wait_ld();
+    if (!live || col >= p.head.n_valid) continue;
+    const int at = h.target - col;
+    if (at >= 0 && at < 64) p.head.target_logit[row] = pick64(f, at);
+    if (col + 64 > p.head.n_valid) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) if (col + j >= p.head.n_valid) f[j] = -INFINITY;
+    }
+    float mx[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      mx[q] = fmaxf(f[q], f[q + 4]);
+#pragma unroll
+      for (int j = 8; j < 64; j += 8) mx[q] = fmax3(mx[q], f[j + q], f[j + q + 4]);
+    }
+    m = fmax3(m, fmax3(mx[0], mx[1], mx[2]), mx[3]);
+  }
+  // a row of nothing but -inf adds nothing; NaN gets into the sum, whatever the maximum says
+  const float ref = m == -INFINITY ? 0.f : m;
+  const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
+#pragma unroll 1
+  for (int c = 0; c < BN; c += 64) {
+    const int col = nb * BN + c;
+    float f[64];
+    tmem_ld32(t_row + c, *(uint32_t(*)[32])&f[0]);
+    tmem_ld32(t_row + c + 32, *(uint32_t(*)[32])&f[32]);
+    tmem_wait_ld();
+    if (c + 64 == BN) release();
+    if (!live || col >= p.N) continue;
+    if (col + 64 > p.head.n_valid) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) if (col + j >= p.head.n_valid) f[j] = -INFINITY;
+    }
+    uint32_t v[32];
+    uint64_t acc[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+#pragma unroll
+    for (int j = 0; j < 64; j += 2) {
+      const uint64_t x = add_f32x2(pack_f32x2(f[j], f[j + 1]), nm);
+      float x0, x1;
+      unpack_f32x2(x, x0, x1);
+      v[j >> 1] = pack_f16(x0, x1);
+      unpack_f32x2(mul_f32x2(x, l2e), x0, x1);
+      acc[(j >> 1) & 1] = add_f32x2(acc[(j >> 1) & 1], pack_f32x2(ex2f(x0), ex2f(x1)));
+    }
+    float a, b;
+    unpack_f32x2(add_f32x2(acc[0], acc[1]), a, b);
+    s += a + b;
+    ws.fill(ws.row_ptr(lane), lane, v);
+    ws.store(tmC, col, row0);
+  }
+  if (row < p.M) p.head.stats[(size_t)nb * p.M + row] = make_float2(m, s);
 }
 
 // Bound by the main loop from a K of about 300 on: a tile's 256 exponentials per thread take the special-function unit 2048 cycles,
@@ -359,6 +429,10 @@ struct GemmLive {
   float* partials;           // workspace of gemm_splits(M, N, K, epi) > 1: as many matrices of M x N floats (accumulating: one less)
   int splits;
 };
+// C fp32 [ranges][M][N], the partial products A w of as many ranges of K as *live.splits says, of at most `most`: A [M, K] and w [K, N]
+// row by row, tiles of `bn` columns.
+int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const Live& live, int* status,
+                    cudaStream_t stream);
 int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t stream);
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream);

@@ -6,9 +6,10 @@
 // (rows_count, rows_gather), and the GEMMs behind read from device memory how many there are (Live in gemm_common.cuh): masked tokens cost
 // nothing, whatever they hold, and the host does not wait for the number.  Then as for the cross entropy (xent.cu): the head's GEMM leaves
 // (max, sum of exponentials) per row and tile of 256 columns, rows_finish makes logp and h of them, and for the gradient a second GEMM
-// computes the logits again or, for wide hidden states, reads the fp32 ones that the first has stored.  Everything per token is
+// computes the logits again or, from a width of 320 on, rows_dlogits takes what the first has kept of them in 16 bits.  Everything per token is
 // computed in 64 bits: e^d - d - 1 of two nearly equal log-probabilities and the sums over long answers need it, and there are few tokens.
 // Every sum has a fixed order: a call repeats bit for bit.
+#include <cuda_fp16.h>
 #include "common.cuh"
 #include "gemm_common.cuh"
 #include "host_utils.h"
@@ -22,8 +23,10 @@ struct Rows {                // the gathered rows, kept from the forward pass to
   int64_t* targets;          // [N] gathered
   float2* norm;              // [N] gathered: (max, 1 / sum of exponentials)
   float* h;                  // [N] gathered: dloss / dlogp, written by the policy loss
+  float* target_p;           // [N] gathered: the target's probability
   __nv_bfloat16* x;          // [N, d] gathered, zero from the last row to the next multiple of 64
-  float* logits;             // [N, V] gathered, or null
+  float2* stats;             // [chunks][tiles][rows of the chunk] (max, sum of exponentials), or null
+  __half* logits;            // [N, V] gathered: distances to the tile's max, or null
 };
 
 __device__ __forceinline__ bool row_counts(const int64_t* targets, const float* weights, int row, int n_valid) {
@@ -149,6 +152,7 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
     if (on) {
       const double lp = logits * ((double)target_logit[row] - (double)m) - log((double)s);
       r.norm[at] = make_float2(m, 1.f / s);
+      r.target_p[at] = (float)exp(lp);
       const int from = r.from[at];
       logp[from] = (float)lp;
       if (POLICY) {
@@ -263,77 +267,137 @@ preference_kernel(const double* __restrict__ sums, int parts, int pairs, const f
   if (threadIdx.x == 0) *loss = (float)l;
 }
 
-// scale = -g dloss/dlogp of the gathered rows, 0 behind the last: what xent.cu calls grad_scale, row by row.  h is by gathered row (each ==
-// 0) or by row / each.
-__global__ void __launch_bounds__(256)
-rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, float* __restrict__ scale, int N) {
-  pdl_release();
-  pdl_wait();
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= N) return;
-  float v = 0.f;
-  if (i < r.live[0]) {
-    v = -(each == 0 ? h[i] : h[r.from[i] / each]);
-    if (g) v *= *g;
+// Into how many ranges of K the product dz w is split: its K is the vocabulary, its tiles are few, and how many there are the host does not
+// know.  The time of the pair with the most work, nanoseconds as in gemm.cu: `t64` for 64 of K, and a write and a read of the partial
+// results in L2 at 16 TB/s.  4600 of 8192 rows, width 384: planned for 8192 rows 222 us, like this 128.
+struct Ranges { int* count; int n_blocks, k_blocks, t64, most, pairs, d; };
+// A whole warp, a candidate per lane (most <= 32).
+__device__ __forceinline__ int ranges_of(const Ranges& q, int rows) {
+  const int tiles = (rows + 2 * GEMM_BM - 1) / (2 * GEMM_BM) * q.n_blocks, s = 1 + (threadIdx.x & 31);
+  const int each = (q.k_blocks + s - 1) / s;
+  float t = 3e38f;
+  if (s <= q.most && (q.k_blocks + each - 1) / each == s)          // no range is empty
+    t = (float)((tiles * s + q.pairs - 1) / q.pairs) * (float)(each * q.t64) + (float)s * (500.f + (float)rows * (float)q.d * (8.f / 16000.f));
+  int at = s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
+    const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
+    if (t2 < t || (t2 == t && at2 < at)) { t = t2; at = at2; }
   }
-  scale[i] = v;
+  return t < 3e38f ? at : 1;
 }
 
-// dlogits of gathered rows from stored logits.  Bound by memory: 4 bytes in and 2 out per logit; four 16-byte loads per thread before the
-// first use.  Rows behind the last one are zero up to the next multiple of 64, see Live.
-constexpr int RD_COLS = 256 * 16;
+// scale = -g dloss/dlogp of the gathered rows, 0 behind the last: what xent.cu calls grad_scale, row by row.  h is by gathered row (each ==
+// 0) or by row / each.  Also the ranges of every chunk of rows.
 __global__ void __launch_bounds__(256)
-rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V, float l2e) {
+rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, float* __restrict__ scale, int N, Ranges q, int chunk) {
+  pdl_release();
+  pdl_wait();
+  const int i = blockIdx.x * 256 + threadIdx.x, live = r.live[0];
+  if (i < N) {
+    float v = 0.f;
+    if (i < live) {
+      v = -(each == 0 ? h[i] : h[r.from[i] / each]);
+      if (g) v *= *g;
+    }
+    scale[i] = v;
+  }
+  const int first = blockIdx.x * 256;                              // a chunk begins with a block
+  if (q.count != nullptr && first % chunk == 0 && threadIdx.x < 32) {
+    const int s = ranges_of(q, max(0, min(chunk, live - first)));
+    if (threadIdx.x == 0) q.count[first / chunk] = s;
+  }
+}
+
+// dlogits of gathered rows from what was kept of the logits.  Bound by memory: 2 bytes in and 2 out per logit; four 16-byte loads per
+// thread before the first use.  Rows behind the last one are zero up to the next multiple of 64, see Live.
+constexpr int RD_COLS = 256 * 32;
+__global__ void __launch_bounds__(256)
+rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, int rows, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V, float l2e) {
   pdl_release();
   pdl_wait();
   const int row = blockIdx.y, at = before + row, live = r.live[0];
   if (at >= ((live + 63) & ~63)) return;
   const float s = scale[at];
   const bool on = s != 0.f;                                        // a row of gradient 0 is zero, whatever its logits are
-  float top = 0.f, inv = 0.f;
-  int64_t tgt = -1;
-  if (on) { top = r.norm[at].x; inv = r.norm[at].y * s; tgt = r.targets[at]; }
-  const int c0 = blockIdx.x * RD_COLS + 4 * threadIdx.x;
-  const float4* x = (const float4*)(r.logits + (size_t)at * V);
-  float4 v[4];
+  const int c0 = blockIdx.x * RD_COLS + 8 * threadIdx.x;
+  uint4 v[4];
+  float f[4];
+  const float2* stats = r.stats + (size_t)((V + 255) / 256) * before + row;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (on && c0 + 1024 * k < V) v[k] = x[(c0 + 1024 * k) >> 2];
+    const int c = c0 + 2048 * k;
+    v[k] = make_uint4(0, 0, 0, 0);
+    f[k] = 0.f;
+    if (on && c < V) {
+      v[k] = *(const uint4*)(r.logits + (size_t)at * V + c);
+      f[k] = stats[(size_t)(c >> 8) * rows].x;
+    }
   }
+  float top = 0.f, inv = 0.f;
+  int tgt = -1;
+  if (on) { top = r.norm[at].x; inv = r.norm[at].y * s; tgt = (int)r.targets[at]; }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int c = c0 + 1024 * k;
+    const int c = c0 + 2048 * k;
     if (c >= V) break;
-    float p[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    const float far = f[k] == -INFINITY ? 0.f : ex2f((f[k] - top) * l2e) * inv;      // a tile of nothing but -inf
+    float p[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      p[e] = on && c + e < n_valid ? ex2f((p[e] - top) * l2e) * inv : 0.f;
-      if (tgt == c + e) p[e] -= s;
+      const float2 d2 = __half22float2(*(const __half2*)&u[e]);
+      p[2 * e] = ex2f(d2.x * l2e) * far;
+      p[2 * e + 1] = ex2f(d2.y * l2e) * far;
     }
-    *(uint2*)(dlogits + (size_t)row * V + c) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+    if (!on || c + 8 > n_valid) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) if (!on || c + e >= n_valid) p[e] = 0.f;
+    }
+    if (tgt >= c && tgt < c + 8) {
+      const float one = s * (r.target_p[at] - 1.f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = tgt == c + e ? one : p[e];
+    }
+    *(uint4*)(dlogits + (size_t)row * V + c) = make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7]));
   }
 }
 
-// dx of every row: the gathered row's, or 0.
+// dx of the rows of one chunk: the gathered row's, the sum of its parts in their order; with the first chunk the rows that do not count, 0.
+// Eight columns per thread, bound by the parts' way through L2.
 __global__ void __launch_bounds__(256)
-rows_scatter_kernel(const __nv_bfloat16* __restrict__ in, const int* __restrict__ place, __nv_bfloat16* __restrict__ out, int N, int d) {
+rows_scatter_kernel(const float* __restrict__ parts, const int* __restrict__ ranges, const int* __restrict__ place, __nv_bfloat16* __restrict__ out,
+                    int N, int d, int before, int rows, size_t total) {
   pdl_release();
   pdl_wait();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, nvec = d >> 3;
-  if (row >= N) return;
-  const int at = place[row];
-  const uint4* src = (const uint4*)(in + (size_t)max(at, 0) * d);
-  uint4* dst = (uint4*)(out + (size_t)row * d);
-  for (int c = lane; c < nvec; c += 128) {
-    uint4 v[4];
+  const int count = *ranges, nvec = d >> 3;
+  const size_t step = (size_t)rows * d / 4;
+  for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    const int row = (int)(i / nvec), c = (int)(i - (size_t)row * nvec), to = place[row], at = to - before;
+    if (to < 0 ? before > 0 : at < 0 || at >= rows) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (to >= 0) {
+      const float4* src = (const float4*)(parts + (size_t)at * d) + 2 * c;
+      a = src[0]; b = src[1];
+      int s = 1;
+      for (; s + 3 < count; s += 4) {
+        float4 u[4], v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = make_uint4(0, 0, 0, 0);
-      if (at >= 0 && c + 32 * k < nvec) v[k] = src[c + 32 * k];
+        for (int k = 0; k < 4; ++k) { u[k] = src[(s + k) * step]; v[k] = src[(s + k) * step + 1]; }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          a.x += u[k].x; a.y += u[k].y; a.z += u[k].z; a.w += u[k].w;
+          b.x += v[k].x; b.y += v[k].y; b.z += v[k].z; b.w += v[k].w;
+        }
+      }
+      for (; s < count; ++s) {
+        const float4 u = src[s * step], v = src[s * step + 1];
+        a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+        b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+      }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) dst[c + 32 * k] = v[k];
+    *(uint4*)(out + (size_t)row * d + 8 * c) = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
   }
 }
 
@@ -371,8 +435,10 @@ static Rows rows_layout(char* base, long N, int d, long V, int store, size_t& by
   r.targets = (int64_t*)(base + take(at, N * 8));
   r.norm = (float2*)(base + take(at, N * 8));
   r.h = (float*)(base + take(at, N * 4));
+  r.target_p = (float*)(base + take(at, N * 4));
   r.x = (__nv_bfloat16*)(base + take(at, (size_t)N * d * 2));
-  r.logits = store ? (float*)(base + take(at, (size_t)N * V * 4)) : nullptr;
+  r.stats = store ? (float2*)(base + take(at, (size_t)((V + 255) / 256) * N * 8)) : nullptr;
+  r.logits = store ? (__half*)(base + take(at, (size_t)N * V * 2)) : nullptr;
   bytes = at;
   return r;
 }
@@ -390,23 +456,38 @@ static FwdScratch fwd_layout(char* base, long N, long V, int chunk, size_t& byte
 }
 // Where dw goes: nowhere, added to an fp32 buffer, or as bf16 (through an fp32 buffer where there are several chunks of rows).
 enum : int { DW_NONE = 0, DW_ADD = 1, DW_BF16 = 2 };
-struct BwdScratch { float* scale; __nv_bfloat16 *dlogits, *dx; float *dw, *partials; size_t partial_bytes; };
+// Tiles of the product dz w: the width that covers d in the least time.  At most 512 MB of partial results.
+static Ranges dx_ranges(int rows, int d, int V) {
+  Ranges q{};
+  long best = 0;
+  for (const int bn : {256, 192, 128}) {
+    const int n = (d + bn - 1) / bn, t64 = bn == 256 ? 370 : bn == 192 ? 300 : 240;
+    if (best == 0 || (long)n * t64 < best) { best = (long)n * t64; q.n_blocks = n; q.t64 = t64; }
+  }
+  q.k_blocks = (V + GEMM_BK - 1) / GEMM_BK;
+  const long most = (128L << 20) / ((long)rows * d);
+  q.most = (int)(most < 2 ? 2 : most > 16 ? 16 : most);
+  q.pairs = sm_count() > 1 ? sm_count() / 2 : 1;
+  q.d = d;
+  return q;
+}
+struct BwdScratch { float* scale; int* ranges; __nv_bfloat16* dlogits; float *dx, *dw, *partials; };
 static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int dw, int want_dx, size_t& bytes) {
   size_t at = 0;
   const long rows = N < chunk ? N : chunk;
   const bool one = N <= chunk;
   BwdScratch s;
   s.scale = (float*)(base + take(at, N * 4));
+  s.ranges = (int*)(base + take(at, (N / chunk + 1) * 4));
   s.dlogits = (__nv_bfloat16*)(base + take(at, (size_t)rows * V * 2));
-  s.dx = (__nv_bfloat16*)(base + take(at, want_dx ? (size_t)N * d * 2 : 0));
   s.dw = (float*)(base + take(at, dw == DW_BF16 && !one ? (size_t)V * d * 4 : 0));
-  size_t most = 0;
+  size_t parts = 0, most = 0;
   for (long r0 = 0; r0 < N; r0 += chunk) {                         // the last chunk has a plan of its own
     const long n = N - r0 < chunk ? N - r0 : chunk;
     if (r0 > 0 && n == chunk) continue;
     if (want_dx) {
-      const int k = gemm_splits((int)n, d, (int)V, EPI_BF16);
-      if (k > 1 && (size_t)k * n * d > most) most = (size_t)k * n * d;
+      const size_t m = (size_t)dx_ranges((int)n, d, (int)V).most * n * d;
+      if (m > parts) parts = m;
     }
     if (dw != DW_NONE) {
       const int epi = dw == DW_BF16 && one ? EPI_BF16 : EPI_F32_ACC, k = gemm_splits((int)V, d, (int)n, epi);
@@ -414,6 +495,7 @@ static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int d
       if (k > 1 && m > most) most = m;
     }
   }
+  s.dx = (float*)(base + take(at, parts * 4));
   s.partials = (float*)(base + take(at, most * 4));
   bytes = at;
   return s;
@@ -463,10 +545,11 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, sums};
   for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
-    const HeadParams head{r.targets + r0, s.stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, (float)(logits * 1.4426950408889634)};
-    if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, store ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, 0, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+    float2* stats = store ? r.stats + (size_t)tiles * r0 : s.stats;
+    const HeadParams head{r.targets + r0, stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, (float)(logits * 1.4426950408889634)};
+    if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, store ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, store ? 2 : 0, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     auto kern = advantages ? rows_finish_kernel<true> : rows_finish_kernel<false>;
-    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, s.stats, s.target_logit, r, logp, r0, n, tiles, logits, q, done, blocks));
+    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, stats, s.target_logit, r, logp, r0, n, tiles, logits, q, done, blocks));
     done += (n + 31) / 32;
   }
   return check_launch("objective_fwd");
@@ -501,32 +584,34 @@ extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, in
   const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, dw_kind, dx != nullptr, bytes);
   const bool one = N <= chunk;
   const float l2e = (float)(logit_scale(d) * 1.4426950408889634);
-  CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h ? h : (const float*)r.h, h ? each : 0, g, s.scale, N));
-  for (int r0 = 0; r0 < N; r0 += chunk) {
+  Ranges q = dx_ranges((int)(one ? N : chunk), d, V);
+  q.count = dx != nullptr ? s.ranges : nullptr;
+  CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h ? h : (const float*)r.h, h ? each : 0, g, s.scale, N, q, chunk));
+  for (int r0 = 0, c = 0; r0 < N; r0 += chunk, ++c) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
     if (store) {
-      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, s.dlogits, n_valid, V, l2e));
+      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, n, s.dlogits, n_valid, V, l2e));
     } else {
       const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0, l2e};
-      if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+      if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     }
     if (dx != nullptr) {
-      GemmLive m{s.dlogits, w, s.dx + (size_t)r0 * d, n, d, V, V, ldw, d, 0, 1, EPI_BF16, s.partials, gemm_splits(n, d, V, EPI_BF16)};
-      if ((rc = gemm_live(m, Live{r.live, r0, 0}, status, stream)) != CPB_OK) return rc;
+      const int bn = q.t64 == 370 ? 256 : q.t64 == 300 ? 192 : 128;
+      if ((rc = gemm_live_parts(s.dlogits, w, s.dx, n, d, V, ldw, bn, q.most, Live{r.live, r0, 0, s.ranges + c}, status, stream)) != CPB_OK) return rc;
+      const size_t total = (size_t)N * (d / 8), blocks = (total + 255) / 256, cap = (size_t)sm_count() * 8;
+      CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, s.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, n, total));
     }
     if (dw_kind != DW_NONE) {
       const bool direct = dw_kind == DW_BF16 && one;
       const int epi = direct ? EPI_BF16 : dw_kind == DW_BF16 && r0 == 0 ? EPI_F32 : EPI_F32_ACC;
       GemmLive m{s.dlogits, r.x + (size_t)r0 * d, dw_kind == DW_BF16 && !one ? (void*)s.dw : dw, V, d, n, V, d, d, 1, 1, epi, s.partials,
                  epi == EPI_F32 ? 1 : gemm_splits(V, d, n, epi)};
-      if ((rc = gemm_live(m, Live{r.live, r0, 1}, status, stream)) != CPB_OK) return rc;
+      if ((rc = gemm_live(m, Live{r.live, r0, 1, nullptr}, status, stream)) != CPB_OK) return rc;
     }
   }
   if (dw_kind == DW_BF16 && !one) {
     const size_t n8 = (size_t)V * d / 8, blocks = (n8 + 255) / 256, cap = (size_t)sm_count() * 8;
     CPB_CUDA_OK(launch_pdl(weight_cast_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, (const float4*)s.dw, (uint4*)dw, n8));
   }
-  if (dx != nullptr)
-    CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (N + 7) / 8, 256, 0, stream, s.dx, r.place, (__nv_bfloat16*)dx, N, d));
   return check_launch("objective_bwd");
 }
