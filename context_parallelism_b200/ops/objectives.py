@@ -75,8 +75,8 @@ def _per_token(name, t, like, optional=False):
 
 # ----------------------------------------------------------------------------- launches
 @functools.lru_cache(maxsize=4096)
-def _plan(N: int, d: int, V: int, chunk: int, store: bool, dw: int, want_dx: bool) -> Tuple[int, int, int]:
-    out = (ctypes.c_int64 * 3)()
+def _plan(N: int, d: int, V: int, chunk: int, store: bool, dw: int, want_dx: bool) -> Tuple[int, int]:
+    out = (ctypes.c_int64 * 2)()
     nv.check(nv.lib().cpb_objective_plan(N, d, V, chunk, store, dw, want_dx, ctypes.addressof(out)), "objective_plan")
     return tuple(out)
 
@@ -118,29 +118,27 @@ def _rows16(t):
 
 
 def _forward(x, w, targets, n_valid, grad, policy=None):
-    """Log-probabilities, what is kept for the backward pass, and for a policy loss its five sums."""
+    """Log-probabilities, what is kept for the backward pass, and for a policy loss the loss and its terms."""
     head = _Head(x, w, targets, n_valid, grad)
     logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
-    sums = None if policy is None else torch.empty(5, dtype=torch.float32, device=x.device)
-    if head.N == 0 or head.d == 0:
-        assert head.N == 0, "hidden states of width 0"
-        return head, None, logp, None if sums is None else sums.zero_()
+    loss = terms = None
+    if policy is not None:
+        loss, terms = torch.empty((), dtype=torch.float32, device=x.device), torch.empty(4, dtype=torch.float32, device=x.device)
+    if head.N == 0:
+        return head, None, logp, loss if loss is None else loss.zero_(), terms if terms is None else terms.zero_()
     xr = x if x.dim() <= 3 and _rows16(x) else x.contiguous() if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.contiguous().clone()
     if xr.dim() == 3:
         T, sb, st = xr.shape[1], xr.stride(0), xr.stride(1)
     else:
         T, sb, st = head.N, 0, xr.stride(-2)
     wr = _weights(w)
-    kept_bytes, scratch_bytes, _ = _plan(head.N, head.d, head.V, head.chunk, head.store, 0, False)
-    kept = torch.empty(kept_bytes, dtype=torch.uint8, device=x.device)
-    scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=x.device)
+    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, 0, False)[0], dtype=torch.uint8, device=x.device)
     old, adv, weights, ref, low, high, kl = policy or (None, None, None, None, 0.0, 0.0, 0.0)
     chunks = -(-head.N // head.chunk)
     nv.LAUNCHES[0] += 1 + 2 * chunks
     nv.call("objective_fwd", xr.data_ptr(), sb, st, head.N, T, head.d, wr.data_ptr(), wr.stride(0), head.V, n_valid, targets.data_ptr(), nv.ptr(old),
-            nv.ptr(adv), nv.ptr(weights), nv.ptr(ref), low, high, kl, logp.data_ptr(), nv.ptr(sums), kept.data_ptr(), head.store, scratch.data_ptr(),
-            head.chunk, nv.status_for(x.device).ptr(), nv.stream_ptr(x.device))
-    return head, kept, logp, sums
+            nv.ptr(adv), nv.ptr(weights), nv.ptr(ref), low, high, kl, logp.data_ptr(), nv.ptr(loss), nv.ptr(terms), kept.data_ptr(), head.store, head.chunk, nv.status_for(x.device).ptr(), nv.stream_ptr(x.device))
+    return head, kept, logp, loss, terms
 
 
 def _weights(w):
@@ -158,8 +156,7 @@ def _backward(head, kept, w, h, each, g, want_dx, want_dw):
             own.zero_()
     elif want_dx or want_dw:
         wr = _weights(w)
-        _, _, scratch_bytes = _plan(head.N, head.d, head.V, head.chunk, head.store, kind, want_dx)
-        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=w.device)
+        scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
         nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, kind, want_dx) - 1
         nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, nv.ptr(g), nv.ptr(dx),
                 (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.store, scratch.data_ptr(), head.chunk,
@@ -175,7 +172,7 @@ def _backward(head, kept, w, h, each, g, want_dx, want_dw):
 class _LogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, n_valid):
-        ctx.head, kept, logp, _ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad))
+        ctx.head, kept, logp, *_ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad))
         ctx.save_for_backward(w, kept)
         return logp
 
@@ -190,9 +187,8 @@ class _LogprobsFn(torch.autograd.Function):
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, n_valid, policy):
-        ctx.head, kept, logp, sums = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad), policy)
+        ctx.head, kept, logp, loss, terms = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad), policy)
         ctx.save_for_backward(w, kept)
-        loss, terms = sums[:1].view(()).clone(), sums[1:]
         ctx.mark_non_differentiable(logp, terms)
         ctx.set_materialize_grads(False)
         return loss, logp, terms
@@ -210,12 +206,12 @@ class _PolicyFn(torch.autograd.Function):
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, n_valid, ref, weights, beta, smoothing, group):
-        ctx.head, kept, logp, _ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad))
+        ctx.head, kept, logp, *_ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad))
         seqs, T = targets.shape
         parts = max(1, -(-T // PART))
         sums = torch.empty((seqs, parts), dtype=torch.float64, device=x.device)
-        out = torch.empty(2 * seqs + 1, dtype=torch.float32, device=x.device)
-        loss, ratios, h = out[:1], out[1:1 + seqs], out[1 + seqs:]
+        loss = torch.empty((), dtype=torch.float32, device=x.device)
+        ratios, h = (torch.empty(seqs, dtype=torch.float32, device=x.device) for _ in range(2))
         stream = nv.stream_ptr(x.device)
         if T:
             nv.call("sequence_sums", logp.data_ptr(), ref.data_ptr(), targets.data_ptr(), sums.data_ptr(), seqs, T, parts, n_valid, stream)
@@ -224,8 +220,7 @@ class _PreferenceFn(torch.autograd.Function):
         if group is not None:
             dist.all_reduce(sums, group=group)
         nv.call("preference", sums.data_ptr(), parts, seqs // 2, nv.ptr(weights), beta, smoothing, loss.data_ptr(), ratios.data_ptr(), h.data_ptr(), stream)
-        ctx.save_for_backward(w, kept, out)
-        loss, ratios = loss.view(()).clone(), ratios.clone()
+        ctx.save_for_backward(w, kept, h)
         ctx.mark_non_differentiable(logp, ratios)
         ctx.set_materialize_grads(False)
         return loss, logp, ratios
@@ -235,9 +230,8 @@ class _PreferenceFn(torch.autograd.Function):
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 9
-        w, kept, out = ctx.saved_tensors
-        seqs, T = ctx.head.shape[:2]
-        dx, dw = _backward(ctx.head, kept, w, out[1 + seqs:], max(1, T), g.float().contiguous(), *ctx.needs_input_grad[:2])
+        w, kept, h = ctx.saved_tensors
+        dx, dw = _backward(ctx.head, kept, w, h, max(1, ctx.head.shape[1]), g.float().contiguous(), *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None, None, None, None, None
 
 

@@ -107,7 +107,7 @@ struct Policy {
   const float *old_logp, *advantages, *weights, *ref_logp;         // [N] by row; weights and ref_logp may be null
   double low, high, kl;                                            // the ratio is clipped to [low, high]
   double* part;                                                    // [blocks][4]
-  float* sums;                                                     // [5] out: loss, then sums of weight x (surrogate, KL, clipped, 1)
+  float *loss, *terms;                                             // [1], and [4] sums of weight x (surrogate, KL, clipped, 1)
 };
 
 // Between the two passes of the head's GEMM: logp and (max, 1 / sum) of 32 gathered rows per block, and for a policy loss its terms and h.
@@ -205,8 +205,8 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
   if (threadIdx.x != 0) return;
   for (int w = 1; w < RF_WARPS; ++w)
     for (int k = 0; k < 4; ++k) total[0][k] += total[w][k];
-  q.sums[0] = (float)(q.ref_logp ? total[0][0] + q.kl * total[0][1] : total[0][0]);
-  for (int k = 0; k < 4; ++k) q.sums[1 + k] = (float)total[0][k];
+  *q.loss = (float)(q.ref_logp ? total[0][0] + q.kl * total[0][1] : total[0][0]);
+  for (int k = 0; k < 4; ++k) q.terms[k] = (float)total[0][k];
 }
 
 // Sums of 256 threads in a fixed order; thread 0 has the result.
@@ -442,13 +442,14 @@ static Rows rows_layout(char* base, long N, int d, long V, int store, size_t& by
   bytes = at;
   return r;
 }
+// What the forward pass alone needs stands behind the rows, in the same buffer: it is small, and an allocation costs the host 3 us.
 struct FwdScratch { int* counts; float2* stats; float* target_logit; double* part; };
-static FwdScratch fwd_layout(char* base, long N, long V, int chunk, size_t& bytes) {
-  size_t at = 0;
+static FwdScratch fwd_layout(char* base, long N, long V, int chunk, int store, size_t& bytes) {
+  size_t at = bytes;
   const long rows = N < chunk ? N : chunk, tiles = (V + 255) / 256;
   FwdScratch s;
   s.counts = (int*)(base + take(at, (N + 31) / 32 * 4));
-  s.stats = (float2*)(base + take(at, (size_t)tiles * rows * 8));
+  s.stats = (float2*)(base + take(at, store ? 0 : (size_t)tiles * rows * 8));
   s.target_logit = (float*)(base + take(at, rows * 4));
   s.part = (double*)(base + take(at, ((N + 31) / 32 + N / chunk + 1) * 32));
   bytes = at;
@@ -505,14 +506,14 @@ static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int d
 
 using namespace cpb;
 
-// Bytes of the buffers of an objective over N rows of width d and V columns: kept between the passes, of the forward pass, of the backward pass.
+// Bytes of the buffers of an objective over N rows of width d and V columns: kept between the passes, and of the backward pass.
 extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int store, int dw, int want_dx, int64_t* bytes) {
   if (N <= 0 || d <= 0 || V <= 0 || chunk <= 0 || chunk % 256) return set_error(CPB_ERR_ARG, "objective: %d rows of %d, %d columns, chunks of %d", N, d, V, chunk);
-  size_t a, b, c;
-  rows_layout(nullptr, N, d, V, store, a);
-  fwd_layout(nullptr, N, V, chunk, b);
-  bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, c);
-  bytes[0] = (int64_t)a; bytes[1] = (int64_t)b; bytes[2] = (int64_t)c;
+  size_t kept, bwd;
+  rows_layout(nullptr, N, d, V, store, kept);
+  fwd_layout(nullptr, N, V, chunk, store, kept);
+  bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, bwd);
+  bytes[0] = (int64_t)kept; bytes[1] = (int64_t)bwd;
   return CPB_OK;
 }
 
@@ -526,23 +527,23 @@ static int objective_args(int N, int d, int V, int n_valid, int ldw, int chunk) 
 
 // x bf16 [B, T, d] (strides sb, st, rows 16-byte aligned), w bf16 [V, d], targets [B, T]; a row counts where 0 <= target < n_valid and, with
 // `weights`, its weight is not 0.  logp [B, T].  With `advantages`, the policy loss: old_logp, advantages, weights, ref_logp [B, T] (the
-// last two may be null) and sums [5], see Policy.  kept and scratch: cpb_objective_plan.
+// last two may be null), loss [1] and terms [4], see Policy.  kept: cpb_objective_plan.
 extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, int d, const void* w, int ldw, int V, int n_valid, const int64_t* targets,
                                  const float* old_logp, const float* advantages, const float* weights, const float* ref_logp, double low, double high,
-                                 double kl, float* logp, float* sums, void* kept, int store, void* scratch, int chunk, int* status, cudaStream_t stream) {
+                                 double kl, float* logp, float* loss, float* terms, void* kept, int store, int chunk, int* status, cudaStream_t stream) {
   int rc = objective_args(N, d, V, n_valid, ldw, chunk);
   if (rc != CPB_OK) return rc;
   if (T <= 0 || N % T || (sb % 8) || (st % 8) || ((uintptr_t)x & 15)) return set_error(CPB_ERR_ARG, "objective: hidden states need 16-byte aligned rows");
   size_t bytes;
   const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
-  const FwdScratch s = fwd_layout((char*)scratch, N, V, chunk, bytes);
+  const FwdScratch s = fwd_layout((char*)kept, N, V, chunk, store, bytes);
   const int groups = (N + 31) / 32, tiles = (V + 255) / 256;
   CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
   CPB_CUDA_OK(launch_pdl(rows_gather_kernel, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, r, N, n_valid));
   int blocks = 0;
   for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
   const double logits = logit_scale(d);
-  const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, sums};
+  const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, loss, terms};
   for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
     float2* stats = store ? r.stats + (size_t)tiles * r0 : s.stats;

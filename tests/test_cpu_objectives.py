@@ -190,10 +190,10 @@ def test_plans():
         chunk = O._chunk(V)
         assert chunk % 256 == 0 and 256 <= chunk <= 65280
         for store in (False, True):
-            kept, fwd, bwd = O._plan(N, d, V, chunk, store, 2, True)
-            assert kept >= N * (4 + 4 + 8 + 8 + 4 + 2 * d + 2 * V * store) and kept % 256 == 0
-            assert fwd >= (V + 255) // 256 * min(N, chunk) * 8 and bwd >= min(N, chunk) * V * 2 + 2 * N * d
-        assert O._plan(N, d, V, chunk, False, 0, False)[2] < bwd
+            kept, bwd = O._plan(N, d, V, chunk, store, 2, True)
+            assert kept >= N * (4 + 4 + 8 + 8 + 4 + 2 * d + 2 * V * store) + (V + 255) // 256 * min(N, chunk) * 8 and kept % 256 == 0
+            assert bwd >= min(N, chunk) * V * 2 + min(N, chunk) * d * 4 * 2
+        assert O._plan(N, d, V, chunk, False, 0, False)[1] < bwd
     for bad in ((0, 8, 8, 256), (1, 0, 8, 256), (1, 8, 0, 256), (1, 8, 8, 0), (1, 8, 8, 100)):
         with pytest.raises(nv.NativeError):
             O._plan(*bad, False, 2, True)
