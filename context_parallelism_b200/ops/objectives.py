@@ -26,10 +26,8 @@ from .gemm import EPI_BF16, EPI_F32_ACC, acc_splits
 
 CHUNK_BYTES = 2 << 30            # of bf16 dlogits, the rows that go through the gradient's products at a time
 KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward to the backward pass
-# Width of the hidden states from which on that is faster than to compute them again.  token_logprobs and its gradient, us, kept and
-# computed again: 4608 x 50304, width 256 567 and 560, 384 664 and 711, 520 1047 and 1153, 768 1001 and 1159, 1024 1245 and 1286; 300 x 50304,
-# 768 199 and 234; 4608 x 8192, 384 199 and 230; 4608 x 128256, 2048 5936 and 7338.
-KEEP_WIDTH = 320
+# Width of the hidden states above which that is faster than to compute them again (and the head's GEMM has an epilogue that does).
+KEEP_ABOVE = 512
 PART = 4096                      # tokens of a sequence that one block adds up
 
 
@@ -109,7 +107,7 @@ class _Head:
         self.shape, self.w, self.n_valid, self.grad = x.shape, w, n_valid, grad
         self.N, self.d, self.V = targets.numel(), x.shape[-1], w.shape[0]
         self.chunk = _chunk(self.V)
-        self.store = grad and self.d >= KEEP_WIDTH and 2 * self.N * self.V <= KEEP_BYTES
+        self.store = grad and self.d > KEEP_ABOVE and 2 * self.N * self.V <= KEEP_BYTES
 
 
 def _rows16(t):

@@ -30,17 +30,17 @@
 
 namespace cpb {
 
-template <int BN>
+template <int BN, int EW = 4>
 struct GemmSmem {
-  static constexpr int STAGES = BN == 384 ? 4 : BN > 128 ? 6 : 8;       // 160 to 192 KB of operands in flight
+  static constexpr int STAGES = EW == 8 ? 5 : BN == 384 ? 4 : BN > 128 ? 6 : 8;       // 160 to 192 KB of operands in flight
   static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2;          // 128 rows of A
   static constexpr int B_GROUPS = (BN / 2 + 63) / 64;            // this CTA's half of B's columns, in groups of 64 (N-major: 96 columns
   static constexpr int B_BYTES = B_GROUPS * 64 * GEMM_BK * 2;    // take two groups, the last 32 columns are loaded and not used)
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int ACCS = BN == 384 ? 1 : 2;                 // accumulators
   static constexpr int ACC_COLS = BN == 384 ? 512 : BN > 128 ? 256 : 128;      // tensor-memory columns of one (a power of two)
-  static constexpr int STORE_OFFSET = STAGES * STAGE_BYTES;      // 4 epilogue warps x 2 buffers x 4 KB
-  static constexpr int BAR_OFFSET = STORE_OFFSET + 32768;
+  static constexpr int STORE_OFFSET = STAGES * STAGE_BYTES;      // epilogue warps x 2 buffers x 4 KB
+  static constexpr int BAR_OFFSET = STORE_OFFSET + EW * 8192;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
 };
 
@@ -115,11 +115,12 @@ __device__ __forceinline__ void pair_tile_coords(int tile, int num_m_tiles, int 
   mt = band * band_rows + (idx - nb * rows);
 }
 
-template <int BN, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+// EW epilogue warps: eight for the head's epilogues of shallow products (head_parts), two for each row, 128 columns each.
+template <int BN, bool A_MN, bool B_MN, int EW = 4>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
 gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmX, GemmParams p) {
-  using L = GemmSmem<BN>;
+  using L = GemmSmem<BN, EW>;
   constexpr int STAGES = L::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -138,7 +139,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&tfull_bar[s], 1); mbar_init(&tempty_bar[s], 8); }      // 4 epilogue warps of each CTA
+    for (int s = 0; s < 2; ++s) { mbar_init(&tfull_bar[s], 1); mbar_init(&tempty_bar[s], 2 * EW); }      // the epilogue warps of both CTAs
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -274,9 +275,9 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
     }
   } else {
-    // ------------------------------------------------------------------ epilogue (warps 2..5 of both CTAs: own 128 rows)
-    const int quarter = warp & 3;
-    WarpStore ws{smem + L::STORE_OFFSET + quarter * 8192, 0u, lane == 0};
+    // ------------------------------------------------------------------ epilogue (warps 2 and up of both CTAs: own 128 rows)
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    WarpStore ws{smem + L::STORE_OFFSET + (half * 4 + quarter) * 8192, 0u, lane == 0};
     int it = 0;
     for (int item = pair; item < num_items; item += num_pairs, ++it) {
       const int acc = L::ACCS == 2 ? it & 1 : 0;
@@ -298,7 +299,8 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           else mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
         }
       };
-      if (p.epi == EPI_HEAD_KEEP) head_keep_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
+      if (EW == 8) head_epilogue<BN / 2>(p, &tmC, ws, t_row + half * (BN / 2), row0, 2 * nb + half, lane, head, release);
+      else if (p.epi == EPI_HEAD_KEEP) head_keep_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
       else if (p.epi >= EPI_HEAD_STATS) head_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
       else gemm_epilogue<BN>(p, &tmC, &tmX, ws, t_row, row0, nb, lane, item / num_tiles, release);
     }
@@ -314,18 +316,18 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
-template <int BN, bool A_MN, bool B_MN>
+template <int BN, bool A_MN, bool B_MN, int EW = 4>
 static int launch_pair(const CUtensorMap (&tm)[4], const GemmParams& p, cudaStream_t stream) {
-  auto kern = gemm_pair_bf16_kernel<BN, A_MN, B_MN>;
+  auto kern = gemm_pair_bf16_kernel<BN, A_MN, B_MN, EW>;
   static bool configured = false;
   if (!configured) {
-    CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmSmem<BN>::TOTAL));
+    CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmSmem<BN, EW>::TOTAL));
     configured = true;
   }
   const int items = p.num_m_tiles * p.num_n_blocks * p.splits;
   const int max_pairs = sm_count() / 2;
   const int pairs = items < max_pairs ? items : max_pairs;
-  CPB_CUDA_OK(launch_pdl(kern, 2 * pairs, GEMM_THREADS, GemmSmem<BN>::TOTAL, stream, tm[0], tm[1], tm[2], tm[3], p));
+  CPB_CUDA_OK(launch_pdl(kern, 2 * pairs, 64 + 32 * EW, GemmSmem<BN, EW>::TOTAL, stream, tm[0], tm[1], tm[2], tm[3], p));
   return check_launch("gemm_pair_bf16");
 }
 
@@ -566,13 +568,13 @@ extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, c
 }
 
 static int gemm_head(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
-                     const Live& live, int* status, cudaStream_t stream) {
+                     const Live& live, bool eight, int* status, cudaStream_t stream) {
   const int n_valid = head.n_valid;
   if (M <= 0 || N <= 0 || K <= 0) return set_error(CPB_ERR_ARG, "gemm_head: empty problem %dx%dx%d", M, N, K);
   if ((N % 8) || (K % 8) || (ldx % 8) || (ldw % 8) || (out && (ldc % 8)))
     return set_error(CPB_ERR_ARG, "gemm_head: N,K,ldx,ldw,ldc must be multiples of 8 (got N=%d K=%d ldx=%d ldw=%d ldc=%d)", N, K, ldx, ldw, ldc);
   if (n_valid <= 0 || n_valid > N) return set_error(CPB_ERR_ARG, "gemm_head: n_valid=%d outside 1..%d", n_valid, N);
-  if (grad == 2 && out == nullptr) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
+  if (grad == 2 && (out == nullptr || eight)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
   if (grad == 1 ? (out == nullptr || head.row_coef == nullptr) : (head.stats == nullptr || head.target_logit == nullptr)) return set_error(CPB_ERR_ARG, "gemm_head: missing buffers");
   GemmParams p{};
   p.M = M; p.N = N; p.K = K; p.epi = grad == 2 ? EPI_HEAD_KEEP : grad ? EPI_HEAD_GRAD : out ? EPI_HEAD_STORE : EPI_HEAD_STATS;
@@ -596,7 +598,7 @@ static int gemm_head(const void* x, const void* w, void* out, int M, int N, int 
     if ((rc = encode_tmap(&tm[2], out, eb, 2, dims, strides, box, 1)) != CPB_OK) return rc;
   }
   tm[3] = tm[2];
-  return launch_pair<256, false, false>(tm, p, stream);
+  return eight ? launch_pair<256, false, false, 8>(tm, p, stream) : launch_pair<256, false, false>(tm, p, stream);
 }
 
 // Cross entropy of the language-model head, logits = x w^T (x [M,K], w [N,K], both K-major).  out == null or fp32 (grad == 0): per row and
@@ -609,7 +611,7 @@ extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int6
                              const float* row_coef, int M, int N, int K, int ldx, int ldw, int ldc, int n_valid, int grad, float grad_scale,
                              int* status, cudaStream_t stream) {
   return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, HeadParams{targets, (float2*)stats, target_logit, (const float2*)row_coef, n_valid, grad_scale, nullptr},
-                   Live{}, status, stream);
+                   Live{}, false, status, stream);
 }
 
 // The same two for objectives.cu, with rows counted on the device.
@@ -619,7 +621,7 @@ int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t str
 }
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream) {
-  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, status, stream);
+  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, head_parts(K) == 2, status, stream);
 }
 int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const Live& live, int* status,
                     cudaStream_t stream) {

@@ -14,7 +14,6 @@ namespace cpb {
 
 constexpr int GEMM_BM = 128;           // rows of A per CTA; a CTA pair computes 256 rows
 constexpr int GEMM_BK = 64;
-constexpr int GEMM_THREADS = 192;
 
 enum : int {
   EPI_BF16 = 0,        // C(bf16) = acc (+bias)
@@ -33,7 +32,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Cross entropy in the epilogue of the head's GEMM (xent.cu has the kernel between the two passes).
 struct HeadParams {
   const int64_t* targets;    // [M]; a row whose target is outside [0, n_valid) has neither loss nor gradient
-  float2* stats;             // [tiles along N][M] (max, sum of exp(x - max))
+  float2* stats;             // [parts][M] (max, sum of exp(x - max)), a part of the columns for each epilogue warp of a row: 256, or 128 of eight warps
   float* target_logit;       // [M], written where the target is in range
   const float2* row_coef;    // [M] (max, grad_scale / sum), (max, 0) for ignored rows; with row_scale (max, 1 / sum)
   int n_valid;               // columns from here on are padding
@@ -167,16 +166,18 @@ __device__ __forceinline__ HeadRow head_row(const GemmParams& p, int row) {
 
 // EPI_HEAD_KEEP: what the backward pass needs of the logits, in 16 bits.  f16 of the distance to the tile's maximum is off by 2^-12 of the
 // distance, so the likely tokens, which are near the maximum, come out of it more exactly than the bf16 that their gradient is rounded to
-// in the end.  The accumulator is read twice, for the maximum and for the rest; the sum of exponentials is that of the fp32 values.
-template <int BN, class Release>
-__device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int nb,
+// in the end.  The accumulator is read twice, for the maximum and for the rest; the sum of exponentials is that of the fp32 values.  "Tile" is
+// the `part` of COLS columns that one warp takes.  With eight warps, five stages of operands are left to the main loop: 274 us, 256 with four
+// (4608 x 50304, K 768).
+template <int COLS, class Release>
+__device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int part,
                                                    int lane, const HeadRow& h, Release release) {
   const int row = row0 + lane;
   const bool live = row0 < p.M;
   float m = -INFINITY, s = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < BN; c += 64) {
-    const int col = nb * BN + c;
+  for (int c = 0; c < COLS; c += 64) {
+    const int col = part * COLS + c;
     float f[64];
     tmem_ld32(t_row + c, *(uint32_t(*)[32])&f[0]);
     tmem_ld32(t_row + c + 32, *(uint32_t(*)[32])&f[32]);
@@ -201,13 +202,13 @@ __device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CU
   const float ref = m == -INFINITY ? 0.f : m;
   const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
 #pragma unroll 1
-  for (int c = 0; c < BN; c += 64) {
-    const int col = nb * BN + c;
+  for (int c = 0; c < COLS; c += 64) {
+    const int col = part * COLS + c;
     float f[64];
     tmem_ld32(t_row + c, *(uint32_t(*)[32])&f[0]);
     tmem_ld32(t_row + c + 32, *(uint32_t(*)[32])&f[32]);
     tmem_wait_ld();
-    if (c + 64 == BN) release();
+    if (c + 64 == COLS) release();
     if (!live || col >= p.N) continue;
     if (col + 64 > p.head.n_valid) {
 #pragma unroll
@@ -230,25 +231,25 @@ __device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CU
     ws.fill(ws.row_ptr(lane), lane, v);
     ws.store(tmC, col, row0);
   }
-  if (row < p.M) p.head.stats[(size_t)nb * p.M + row] = make_float2(m, s);
+  if (row < p.M) p.head.stats[(size_t)part * p.M + row] = make_float2(m, s);
 }
 
 // Bound by the main loop from a K of about 300 on: a tile's 256 exponentials per thread take the special-function unit 2048 cycles,
 // 64 of K take 370 ns.
-template <int BN, class Release>
-__device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int nb,
+template <int COLS, class Release>
+__device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int part,
                                               int lane, const HeadRow& h, Release release) {
   const int row = row0 + lane;
   const bool live = row0 < p.M;
   float m = -INFINITY, s = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < BN; c += 64) {
-    const int col = nb * BN + c;
+  for (int c = 0; c < COLS; c += 64) {
+    const int col = part * COLS + c;
     float f[64];
     tmem_ld32(t_row + c, *(uint32_t(*)[32])&f[0]);
     tmem_ld32(t_row + c + 32, *(uint32_t(*)[32])&f[32]);
     tmem_wait_ld();
-    if (c + 64 == BN) release();
+    if (c + 64 == COLS) release();
     if (!live || col >= p.N) continue;
     const int at = h.target - col;
     const bool hit = at >= 0 && at < 64;
@@ -316,7 +317,7 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
       ws.store(tmC, col, row0);
     }
   }
-  if (p.epi != EPI_HEAD_GRAD && row < p.M) p.head.stats[(size_t)nb * p.M + row] = make_float2(m, s);
+  if (p.epi != EPI_HEAD_GRAD && row < p.M) p.head.stats[(size_t)part * p.M + row] = make_float2(m, s);
 }
 
 // Epilogue of one 32-row slice of a 128 x BN accumulator tile: `t_row` is the tensor-memory address of this warp's lanes at
@@ -420,6 +421,10 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
     }
   }
 }
+
+// Into how many parts the objectives' head splits the 256 columns of a row, an epilogue warp each.  Up to a K of 512 the exponentials take longer
+// than the main loop.  us at 4608 x 50304 with one and two: K 384 statistics 160 and 138, gradient 196 and 176, K 768 217 and 226, 263 and 268.
+constexpr int head_parts(int K) { return K <= 512 ? 2 : 1; }
 
 // gemm.cu, for objectives.cu
 struct GemmLive {

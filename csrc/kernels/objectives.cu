@@ -5,8 +5,8 @@
 // Of a fine-tuning batch only the answers' tokens count, a third to two thirds of it.  So the counted rows are gathered first, in their order
 // (rows_count, rows_gather), and the GEMMs behind read from device memory how many there are (Live in gemm_common.cuh): masked tokens cost
 // nothing, whatever they hold, and the host does not wait for the number.  Then as for the cross entropy (xent.cu): the head's GEMM leaves
-// (max, sum of exponentials) per row and tile of 256 columns, rows_finish makes logp and h of them, and for the gradient a second GEMM
-// computes the logits again or, from a width of 320 on, rows_dlogits takes what the first has kept of them in 16 bits.  Everything per token is
+// (max, sum of exponentials) per row and part of the columns, rows_finish makes logp and h of them, and for the gradient a second GEMM
+// computes the logits again or, from a width of 520 on, rows_dlogits takes what the first has kept of them in 16 bits.  Everything per token is
 // computed in 64 bits: e^d - d - 1 of two nearly equal log-probabilities and the sums over long answers need it, and there are few tokens.
 // Every sum has a fixed order: a call repeats bit for bit.
 #include <cuda_fp16.h>
@@ -25,8 +25,8 @@ struct Rows {                // the gathered rows, kept from the forward pass to
   float* h;                  // [N] gathered: dloss / dlogp, written by the policy loss
   float* target_p;           // [N] gathered: the target's probability
   __nv_bfloat16* x;          // [N, d] gathered, zero from the last row to the next multiple of 64
-  float2* stats;             // [chunks][tiles][rows of the chunk] (max, sum of exponentials), or null
-  __half* logits;            // [N, V] gathered: distances to the tile's max, or null
+  float2* stats;             // [chunks][parts][rows of the chunk] (max, sum of exponentials), or null
+  __half* logits;            // [N, V] gathered: distances to the part's max, or null
 };
 
 __device__ __forceinline__ bool row_counts(const int64_t* targets, const float* weights, int row, int n_valid) {
@@ -444,12 +444,12 @@ static Rows rows_layout(char* base, long N, int d, long V, int store, size_t& by
 }
 // What the forward pass alone needs stands behind the rows, in the same buffer: it is small, and an allocation costs the host 3 us.
 struct FwdScratch { int* counts; float2* stats; float* target_logit; double* part; };
-static FwdScratch fwd_layout(char* base, long N, long V, int chunk, int store, size_t& bytes) {
+static FwdScratch fwd_layout(char* base, long N, int d, long V, int chunk, int store, size_t& bytes) {
   size_t at = bytes;
-  const long rows = N < chunk ? N : chunk, tiles = (V + 255) / 256;
+  const long rows = N < chunk ? N : chunk, parts = (V + 255) / 256 * head_parts(d);
   FwdScratch s;
   s.counts = (int*)(base + take(at, (N + 31) / 32 * 4));
-  s.stats = (float2*)(base + take(at, store ? 0 : (size_t)tiles * rows * 8));
+  s.stats = (float2*)(base + take(at, store ? 0 : (size_t)parts * rows * 8));
   s.target_logit = (float*)(base + take(at, rows * 4));
   s.part = (double*)(base + take(at, ((N + 31) / 32 + N / chunk + 1) * 32));
   bytes = at;
@@ -511,7 +511,7 @@ extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int store, int
   if (N <= 0 || d <= 0 || V <= 0 || chunk <= 0 || chunk % 256) return set_error(CPB_ERR_ARG, "objective: %d rows of %d, %d columns, chunks of %d", N, d, V, chunk);
   size_t kept, bwd;
   rows_layout(nullptr, N, d, V, store, kept);
-  fwd_layout(nullptr, N, V, chunk, store, kept);
+  fwd_layout(nullptr, N, d, V, chunk, store, kept);
   bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, bwd);
   bytes[0] = (int64_t)kept; bytes[1] = (int64_t)bwd;
   return CPB_OK;
@@ -536,8 +536,8 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   if (T <= 0 || N % T || (sb % 8) || (st % 8) || ((uintptr_t)x & 15)) return set_error(CPB_ERR_ARG, "objective: hidden states need 16-byte aligned rows");
   size_t bytes;
   const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
-  const FwdScratch s = fwd_layout((char*)kept, N, V, chunk, store, bytes);
-  const int groups = (N + 31) / 32, tiles = (V + 255) / 256;
+  const FwdScratch s = fwd_layout((char*)kept, N, d, V, chunk, store, bytes);
+  const int groups = (N + 31) / 32, tiles = (V + 255) / 256 * head_parts(d);
   CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
   CPB_CUDA_OK(launch_pdl(rows_gather_kernel, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, r, N, n_valid));
   int blocks = 0;

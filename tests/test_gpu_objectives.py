@@ -45,7 +45,7 @@ class _Exact:
         self.p = lp.exp()
         # From a width on, the distance of a logit to its tile's maximum is kept in f16, half a step 2^-11 of the distance, which is no more than
         # that to the row's maximum: the probability changes by a factor of e to that at most, (1 + 2 x) for x below a half.
-        self.kept = (2 * 2.0 ** -11 * (z.amax(1, keepdim=True) - z)).clamp(max=1) if x.shape[-1] >= O.KEEP_WIDTH and O.KEEP_BYTES else 0.0 * z
+        self.kept = (2 * 2.0 ** -11 * (z.amax(1, keepdim=True) - z)).clamp(max=1) if x.shape[-1] > O.KEEP_ABOVE and O.KEEP_BYTES else 0.0 * z
         self.logp = torch.where(self.on, lp.gather(1, self.t.clamp(min=0)[:, None])[:, 0], 0.0)
         self.V, self.shape = w.shape[0], x.shape
 
