@@ -29,6 +29,7 @@ KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward t
 # Width of the hidden states above which that is faster than to compute them again (and the head's GEMM has an epilogue that does).
 KEEP_ABOVE = 512
 PART = 4096                      # tokens of a sequence that one block adds up
+COUNT_ROWS = 4096                # up to which rows are counted and gathered in one launch
 
 
 class PolicyLoss(NamedTuple):
@@ -133,7 +134,7 @@ def _forward(x, w, targets, n_valid, grad, policy=None):
     kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, 0, False)[0], dtype=torch.uint8, device=x.device)
     old, adv, weights, ref, low, high, kl = policy or (None, None, None, None, 0.0, 0.0, 0.0)
     chunks = -(-head.N // head.chunk)
-    nv.LAUNCHES[0] += 1 + 2 * chunks
+    nv.LAUNCHES[0] += (head.N > COUNT_ROWS) + 2 * chunks
     nv.call("objective_fwd", xr.data_ptr(), sb, st, head.N, T, head.d, wr.data_ptr(), wr.stride(0), head.V, n_valid, targets.data_ptr(), nv.ptr(old),
             nv.ptr(adv), nv.ptr(weights), nv.ptr(ref), low, high, kl, logp.data_ptr(), nv.ptr(loss), nv.ptr(terms), kept.data_ptr(), head.store, head.chunk, nv.status_for(x.device).ptr(), nv.stream_ptr(x.device))
     return head, kept, logp, loss, terms
@@ -155,7 +156,7 @@ def _backward(head, kept, w, h, each, g, want_dx, want_dw):
     elif want_dx or want_dw:
         wr = _weights(w)
         scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
-        nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, kind, want_dx) - 1
+        nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, kind, want_dx) - head.store - 1
         nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, nv.ptr(g), nv.ptr(dx),
                 (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.store, scratch.data_ptr(), head.chunk,
                 nv.status_for(w.device).ptr(), nv.stream_ptr(w.device))
@@ -211,13 +212,17 @@ class _PreferenceFn(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=x.device)
         ratios, h = (torch.empty(seqs, dtype=torch.float32, device=x.device) for _ in range(2))
         stream = nv.stream_ptr(x.device)
-        if T:
-            nv.call("sequence_sums", logp.data_ptr(), ref.data_ptr(), targets.data_ptr(), sums.data_ptr(), seqs, T, parts, n_valid, stream)
-        else:
+        mine = (logp.data_ptr(), ref.data_ptr(), targets.data_ptr())
+        if T == 0:
             sums.zero_()
+        elif group is not None:
+            nv.call("sequence_sums", *mine, sums.data_ptr(), seqs, T, parts, n_valid, stream)
+        else:
+            nv.LAUNCHES[0] += 1
         if group is not None:
             dist.all_reduce(sums, group=group)
-        nv.call("preference", sums.data_ptr(), parts, seqs // 2, nv.ptr(weights), beta, smoothing, loss.data_ptr(), ratios.data_ptr(), h.data_ptr(), stream)
+        nv.call("preference", *(mine if T and group is None else (0, 0, 0)), T, n_valid, sums.data_ptr(), parts, seqs // 2, nv.ptr(weights), beta, smoothing,
+                loss.data_ptr(), ratios.data_ptr(), h.data_ptr(), stream)
         ctx.save_for_backward(w, kept, h)
         ctx.mark_non_differentiable(logp, ratios)
         ctx.set_materialize_grads(False)

@@ -18,6 +18,7 @@ namespace cpb {
 
 struct Rows {                // the gathered rows, kept from the forward pass to the backward pass
   int* live;                 // [0] how many, [1] a ticket
+  int* ranges;               // [chunks] into how many ranges of K the product for dx is split
   int* from;                 // [N] gathered row -> row
   int* place;                // [N] row -> gathered row, or -1
   int64_t* targets;          // [N] gathered
@@ -52,16 +53,45 @@ rows_count_kernel(const int64_t* __restrict__ targets, const float* __restrict__
   if (row == 0) live[1] = 0;
 }
 
-// Gathers 32 rows per block: x[b, t] has strides sb and st.  Bound by memory, 2 d bytes in and out per row.
+// Into how many ranges of K the product dz w is split: its K is the vocabulary, its tiles are few, and how many there are the host does not
+// know.  The time of the pair with the most work, nanoseconds as in gemm.cu: `t64` for 64 of K, and a write and a read of the partial
+// results in L2 at 16 TB/s.  4600 of 8192 rows, width 384: planned for 8192 rows 222 us, like this 128.
+struct Ranges { int n_blocks, k_blocks, t64, most, pairs, d; };
+// A whole warp, a candidate per lane (most <= 32).
+__device__ __forceinline__ int ranges_of(const Ranges& q, int rows) {
+  const int tiles = (rows + 2 * GEMM_BM - 1) / (2 * GEMM_BM) * q.n_blocks, s = 1 + (threadIdx.x & 31);
+  const int each = (q.k_blocks + s - 1) / s;
+  float t = 3e38f;
+  if (s <= q.most && (q.k_blocks + each - 1) / each == s)          // no range is empty
+    t = (float)((tiles * s + q.pairs - 1) / q.pairs) * (float)(each * q.t64) + (float)s * (200.f + (float)rows * (float)q.d * (8.f / 16000.f));
+  int at = s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
+    const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
+    if (t2 < t || (t2 == t && at2 < at)) { t = t2; at = at2; }
+  }
+  return t < 3e38f ? at : 1;
+}
+
+// Gathers 32 rows per block: x[b, t] has strides sb and st.  Bound by memory, 2 d bytes in and out per row.  COUNT: every block counts the
+// rows in front of its own by itself and there is no rows_count, up to COUNT_ROWS rows: 136 rows of 768 11 us for both kernels, 7 for one.
+constexpr int COUNT_ROWS = 4096;
+template <bool COUNT>
 __global__ void __launch_bounds__(256)
 rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T, int d, const int64_t* __restrict__ targets,
-                   const float* __restrict__ weights, const int* __restrict__ counts, Rows r, int N, int n_valid) {
+                   const float* __restrict__ weights, const int* __restrict__ counts, float* __restrict__ logp, Rows r, Ranges q, int chunk, int N, int n_valid,
+                   int* status) {
   pdl_release();
   pdl_wait();
   __shared__ int part[8], s_base, s_n, s_from[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x;
   int before = 0;
-  for (int i = threadIdx.x; i < group; i += 256) before += counts[i];
+  if (COUNT) {
+    for (int i = threadIdx.x; i < group * 32; i += 256) before += row_counts(targets, weights, i, n_valid);
+  } else {
+    for (int i = threadIdx.x; i < group; i += 256) before += counts[i];
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if (lane == 0) part[warp] = before;
@@ -79,8 +109,19 @@ rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T,
       r.targets[base + rank] = targets[row];
     }
     if (row < N) r.place[row] = on ? base + rank : -1;
+    if (COUNT && row < N) {
+      logp[row] = 0.f;
+      if (targets[row] >= n_valid) report(status, ST_BAD_INDEX, 1300, (int)targets[row]);
+    }
     if (lane == 0) { s_base = base; s_n = __popc(mask); }
-    if (lane == 0 && group == (int)gridDim.x - 1) r.live[0] = base + __popc(mask);
+    if (group == (int)gridDim.x - 1) {
+      const int live = base + __popc(mask);
+      if (lane == 0) { r.live[0] = live; if (COUNT) r.live[1] = 0; }
+      for (int c = 0; c * chunk < N; ++c) {
+        const int s = ranges_of(q, max(0, min(chunk, live - c * chunk)));
+        if (lane == 0) r.ranges[c] = s;
+      }
+    }
   }
   __syncthreads();
   const int nvec = d >> 3;
@@ -111,8 +152,8 @@ struct Policy {
 };
 
 // Between the two passes of the head's GEMM: logp and (max, 1 / sum) of 32 gathered rows per block, and for a policy loss its terms and h.
-// A warp takes every eighth tile (the lanes' pairs are adjacent in memory), warp 0 adds the eight parts, always in the same order.
-constexpr int RF_WARPS = 8;
+// A warp takes every sixteenth part of the columns (the lanes' pairs are adjacent in memory), warp 0 adds the warps', always in the same order.
+constexpr int RF_WARPS = 16;
 template <bool POLICY>
 __global__ void __launch_bounds__(RF_WARPS * 32)
 rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logit, Rows r, float* __restrict__ logp, int before, int rows,
@@ -135,12 +176,12 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
   };
   if (on) {
     int t = warp;
-    for (; t + 3 * RF_WARPS < tiles; t += 4 * RF_WARPS) {
-      float2 v[4];
+    for (; t + 7 * RF_WARPS < tiles; t += 8 * RF_WARPS) {
+      float2 v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = stats[(size_t)(t + k * RF_WARPS) * rows + row];
+      for (int k = 0; k < 8; ++k) v[k] = stats[(size_t)(t + k * RF_WARPS) * rows + row];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) add(v[k]);
+      for (int k = 0; k < 8; ++k) add(v[k]);
     }
     for (; t < tiles; t += RF_WARPS) add(stats[(size_t)t * rows + row]);
   }
@@ -267,59 +308,30 @@ preference_kernel(const double* __restrict__ sums, int parts, int pairs, const f
   if (threadIdx.x == 0) *loss = (float)l;
 }
 
-// Into how many ranges of K the product dz w is split: its K is the vocabulary, its tiles are few, and how many there are the host does not
-// know.  The time of the pair with the most work, nanoseconds as in gemm.cu: `t64` for 64 of K, and a write and a read of the partial
-// results in L2 at 16 TB/s.  4600 of 8192 rows, width 384: planned for 8192 rows 222 us, like this 128.
-struct Ranges { int* count; int n_blocks, k_blocks, t64, most, pairs, d; };
-// A whole warp, a candidate per lane (most <= 32).
-__device__ __forceinline__ int ranges_of(const Ranges& q, int rows) {
-  const int tiles = (rows + 2 * GEMM_BM - 1) / (2 * GEMM_BM) * q.n_blocks, s = 1 + (threadIdx.x & 31);
-  const int each = (q.k_blocks + s - 1) / s;
-  float t = 3e38f;
-  if (s <= q.most && (q.k_blocks + each - 1) / each == s)          // no range is empty
-    t = (float)((tiles * s + q.pairs - 1) / q.pairs) * (float)(each * q.t64) + (float)s * (500.f + (float)rows * (float)q.d * (8.f / 16000.f));
-  int at = s;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
-    const int at2 = __shfl_xor_sync(0xffffffffu, at, o);
-    if (t2 < t || (t2 == t && at2 < at)) { t = t2; at = at2; }
-  }
-  return t < 3e38f ? at : 1;
-}
-
 // scale = -g dloss/dlogp of the gathered rows, 0 behind the last: what xent.cu calls grad_scale, row by row.  h is by gathered row (each ==
-// 0) or by row / each.  Also the ranges of every chunk of rows.
+// 0) or by row / each.
+__device__ __forceinline__ float row_scale(const Rows& r, const float* __restrict__ h, int each, const float* __restrict__ g, int i) {
+  const float v = -(each == 0 ? h[i] : h[r.from[i] / each]);
+  return g ? v * *g : v;
+}
 __global__ void __launch_bounds__(256)
-rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, float* __restrict__ scale, int N, Ranges q, int chunk) {
+rows_scale_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, float* __restrict__ scale, int N) {
   pdl_release();
   pdl_wait();
-  const int i = blockIdx.x * 256 + threadIdx.x, live = r.live[0];
-  if (i < N) {
-    float v = 0.f;
-    if (i < live) {
-      v = -(each == 0 ? h[i] : h[r.from[i] / each]);
-      if (g) v *= *g;
-    }
-    scale[i] = v;
-  }
-  const int first = blockIdx.x * 256;                              // a chunk begins with a block
-  if (q.count != nullptr && first % chunk == 0 && threadIdx.x < 32) {
-    const int s = ranges_of(q, max(0, min(chunk, live - first)));
-    if (threadIdx.x == 0) q.count[first / chunk] = s;
-  }
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < N) scale[i] = i < r.live[0] ? row_scale(r, h, each, g, i) : 0.f;
 }
 
 // dlogits of gathered rows from what was kept of the logits.  Bound by memory: 2 bytes in and 2 out per logit; four 16-byte loads per
 // thread before the first use.  Rows behind the last one are zero up to the next multiple of 64, see Live.
 constexpr int RD_COLS = 256 * 32;
 __global__ void __launch_bounds__(256)
-rows_dlogits_kernel(Rows r, const float* __restrict__ scale, int before, int rows, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V, float l2e) {
+rows_dlogits_kernel(Rows r, const float* __restrict__ h, int each, const float* __restrict__ g, int before, int rows, __nv_bfloat16* __restrict__ dlogits, int n_valid, int V, float l2e) {
   pdl_release();
   pdl_wait();
   const int row = blockIdx.y, at = before + row, live = r.live[0];
   if (at >= ((live + 63) & ~63)) return;
-  const float s = scale[at];
+  const float s = at < live ? row_scale(r, h, each, g, at) : 0.f;
   const bool on = s != 0.f;                                        // a row of gradient 0 is zero, whatever its logits are
   const int c0 = blockIdx.x * RD_COLS + 8 * threadIdx.x;
   uint4 v[4];
@@ -426,10 +438,11 @@ static size_t take(size_t& at, size_t bytes) {
   return here;
 }
 // `base` may be null: the size alone
-static Rows rows_layout(char* base, long N, int d, long V, int store, size_t& bytes) {
+static Rows rows_layout(char* base, long N, int d, long V, int chunk, int store, size_t& bytes) {
   size_t at = 0;
   Rows r;
   r.live = (int*)(base + take(at, 256));
+  r.ranges = (int*)(base + take(at, (N / chunk + 1) * 4));
   r.from = (int*)(base + take(at, N * 4));
   r.place = (int*)(base + take(at, N * 4));
   r.targets = (int64_t*)(base + take(at, N * 8));
@@ -467,19 +480,18 @@ static Ranges dx_ranges(int rows, int d, int V) {
   }
   q.k_blocks = (V + GEMM_BK - 1) / GEMM_BK;
   const long most = (128L << 20) / ((long)rows * d);
-  q.most = (int)(most < 2 ? 2 : most > 16 ? 16 : most);
+  q.most = (int)(most < 2 ? 2 : most > 32 ? 32 : most);
   q.pairs = sm_count() > 1 ? sm_count() / 2 : 1;
   q.d = d;
   return q;
 }
-struct BwdScratch { float* scale; int* ranges; __nv_bfloat16* dlogits; float *dx, *dw, *partials; };
+struct BwdScratch { float* scale; __nv_bfloat16* dlogits; float *dx, *dw, *partials; };
 static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int dw, int want_dx, size_t& bytes) {
   size_t at = 0;
   const long rows = N < chunk ? N : chunk;
   const bool one = N <= chunk;
   BwdScratch s;
   s.scale = (float*)(base + take(at, N * 4));
-  s.ranges = (int*)(base + take(at, (N / chunk + 1) * 4));
   s.dlogits = (__nv_bfloat16*)(base + take(at, (size_t)rows * V * 2));
   s.dw = (float*)(base + take(at, dw == DW_BF16 && !one ? (size_t)V * d * 4 : 0));
   size_t parts = 0, most = 0;
@@ -510,7 +522,7 @@ using namespace cpb;
 extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int store, int dw, int want_dx, int64_t* bytes) {
   if (N <= 0 || d <= 0 || V <= 0 || chunk <= 0 || chunk % 256) return set_error(CPB_ERR_ARG, "objective: %d rows of %d, %d columns, chunks of %d", N, d, V, chunk);
   size_t kept, bwd;
-  rows_layout(nullptr, N, d, V, store, kept);
+  rows_layout(nullptr, N, d, V, chunk, store, kept);
   fwd_layout(nullptr, N, d, V, chunk, store, kept);
   bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, bwd);
   bytes[0] = (int64_t)kept; bytes[1] = (int64_t)bwd;
@@ -535,11 +547,14 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   if (rc != CPB_OK) return rc;
   if (T <= 0 || N % T || (sb % 8) || (st % 8) || ((uintptr_t)x & 15)) return set_error(CPB_ERR_ARG, "objective: hidden states need 16-byte aligned rows");
   size_t bytes;
-  const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
+  const Rows r = rows_layout((char*)kept, N, d, V, chunk, store, bytes);
   const FwdScratch s = fwd_layout((char*)kept, N, d, V, chunk, store, bytes);
   const int groups = (N + 31) / 32, tiles = (V + 255) / 256 * head_parts(d);
-  CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
-  CPB_CUDA_OK(launch_pdl(rows_gather_kernel, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, r, N, n_valid));
+  const bool count = N <= COUNT_ROWS;
+  if (!count) CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
+  auto gather = count ? rows_gather_kernel<true> : rows_gather_kernel<false>;
+  CPB_CUDA_OK(launch_pdl(gather, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, logp, r, dx_ranges(N < chunk ? N : chunk, d, V),
+                         chunk, N, n_valid, status));
   int blocks = 0;
   for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
   const double logits = logit_scale(d);
@@ -557,16 +572,24 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
 }
 
 // sums fp64 [2 pairs][parts] of logp - ref over the counted tokens of every sequence of T tokens, part by part.
-extern "C" int cpb_sequence_sums(const float* logp, const float* ref, const int64_t* targets, double* sums, int seqs, int T, int parts, int n_valid,
-                                 cudaStream_t stream) {
+static int sequence_sums(const float* logp, const float* ref, const int64_t* targets, double* sums, int seqs, int T, int parts, int n_valid,
+                         cudaStream_t stream) {
   if (seqs <= 0 || T <= 0 || parts <= 0 || seqs > 65535) return set_error(CPB_ERR_ARG, "sequence_sums: %d sequences of %d in %d parts", seqs, T, parts);
   CPB_CUDA_OK(launch_pdl(sequence_sums_kernel, dim3(parts, seqs), 256, 0, stream, logp, ref, targets, sums, T, (T + parts - 1) / parts, n_valid));
   return check_launch("sequence_sums");
 }
+extern "C" int cpb_sequence_sums(const float* logp, const float* ref, const int64_t* targets, double* sums, int seqs, int T, int parts, int n_valid,
+                                 cudaStream_t stream) {
+  return sequence_sums(logp, ref, targets, sums, seqs, T, parts, n_valid, stream);
+}
 
-// loss [1], ratios [2 pairs] and h [2 pairs] from the sums; weights [pairs] or null.
-extern "C" int cpb_preference(const double* sums, int parts, int pairs, const float* weights, double beta, double smoothing, float* loss, float* ratios,
-                              float* h, cudaStream_t stream) {
+// loss [1], ratios [2 pairs] and h [2 pairs] from the sums, which with `logp` are taken first; weights [pairs] or null.
+extern "C" int cpb_preference(const float* logp, const float* ref, const int64_t* targets, int T, int n_valid, double* sums, int parts, int pairs,
+                              const float* weights, double beta, double smoothing, float* loss, float* ratios, float* h, cudaStream_t stream) {
+  if (logp != nullptr) {
+    const int rc = sequence_sums(logp, ref, targets, sums, 2 * pairs, T, parts, n_valid, stream);
+    if (rc != CPB_OK) return rc;
+  }
   if (pairs <= 0 || parts <= 0) return set_error(CPB_ERR_ARG, "preference: %d pairs in %d parts", pairs, parts);
   CPB_CUDA_OK(launch_pdl(preference_kernel, 1, 256, 0, stream, sums, parts, pairs, weights, beta, smoothing, loss, ratios, h));
   return check_launch("preference");
@@ -581,26 +604,26 @@ extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, in
   if ((h != nullptr && each <= 0) || dw_kind < DW_NONE || dw_kind > DW_BF16 || (dw_kind != DW_NONE && dw == nullptr))
     return set_error(CPB_ERR_ARG, "objective: gradients of %d rows each, weights' gradient of kind %d", each, dw_kind);
   size_t bytes;
-  const Rows r = rows_layout((char*)kept, N, d, V, store, bytes);
+  const Rows r = rows_layout((char*)kept, N, d, V, chunk, store, bytes);
   const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, dw_kind, dx != nullptr, bytes);
   const bool one = N <= chunk;
   const float l2e = (float)(logit_scale(d) * 1.4426950408889634);
-  Ranges q = dx_ranges((int)(one ? N : chunk), d, V);
-  q.count = dx != nullptr ? s.ranges : nullptr;
-  CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h ? h : (const float*)r.h, h ? each : 0, g, s.scale, N, q, chunk));
+  const Ranges q = dx_ranges(one ? N : chunk, d, V);
+  if (h == nullptr) { h = r.h; each = 0; }
+  if (!store) CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h, each, g, s.scale, N));
   for (int r0 = 0, c = 0; r0 < N; r0 += chunk, ++c) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
     if (store) {
-      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, s.scale, r0, n, s.dlogits, n_valid, V, l2e));
+      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, h, each, g, r0, n, s.dlogits, n_valid, V, l2e));
     } else {
       const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0, l2e};
       if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     }
     if (dx != nullptr) {
       const int bn = q.t64 == 370 ? 256 : q.t64 == 300 ? 192 : 128;
-      if ((rc = gemm_live_parts(s.dlogits, w, s.dx, n, d, V, ldw, bn, q.most, Live{r.live, r0, 0, s.ranges + c}, status, stream)) != CPB_OK) return rc;
+      if ((rc = gemm_live_parts(s.dlogits, w, s.dx, n, d, V, ldw, bn, q.most, Live{r.live, r0, 0, r.ranges + c}, status, stream)) != CPB_OK) return rc;
       const size_t total = (size_t)N * (d / 8), blocks = (total + 255) / 256, cap = (size_t)sm_count() * 8;
-      CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, s.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, n, total));
+      CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, r.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, n, total));
     }
     if (dw_kind != DW_NONE) {
       const bool direct = dw_kind == DW_BF16 && one;
