@@ -191,6 +191,12 @@ __device__ __forceinline__ void bulk_load_1d(void* smem, const void* gmem, uint3
                ::"r"(smem_u32(smem)), "l"((uint64_t)gmem), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 // A global load that stays where it is written (the compiler would otherwise sink it to its first use, one tile later).
+// A thread's own copies to shared memory, which only it reads: 16 bytes each, in groups.
+__device__ __forceinline__ void copy_ahead16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void copy_ahead_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_ahead_wait1() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }      // all but the newest group
 __device__ __forceinline__ int ld_ahead_s32(const int* ptr) {
   int v;
   asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(ptr));

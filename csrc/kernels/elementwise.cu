@@ -64,38 +64,74 @@ __device__ __forceinline__ uint64_t drop_row(const Drop& q, unsigned row) {
   const unsigned b = row / (unsigned)q.T, t = row - b * (unsigned)q.T;
   return (uint64_t)b * (uint64_t)q.seq_len + (uint64_t)(q.pos ? q.pos[t] : (int64_t)t);
 }
-__device__ __forceinline__ uint4 philox7(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, DropKey k) {
+constexpr uint32_t PHILOX_M0 = 0xD2511F53u, PHILOX_M1 = 0xCD9E8D57u, PHILOX_W0 = 0x9E3779B9u, PHILOX_W1 = 0xBB67AE85u;
+// Bound by the 32 x 32 -> 64 bit products, two a round.  The counter's row and column first meet in the third round: what the first two make
+// of the row is taken once per row, what they make of the column once for the rows that a thread takes of it.
+struct DropRow { uint32_t x, hi, lo; };
+__device__ __forceinline__ DropRow drop_row_part(const Drop& q, DropKey k, unsigned row) {
+  const uint64_t place = drop_row(q, row);
+  const uint64_t b = (uint64_t)(uint32_t)(place >> 32) * PHILOX_M1;
+  const uint64_t a = (uint64_t)((uint32_t)(b >> 32) ^ (uint32_t)place ^ k.k0) * PHILOX_M0;
+  return DropRow{(uint32_t)b ^ (k.k0 + PHILOX_W0), (uint32_t)(a >> 32) ^ (k.k1 + PHILOX_W1), (uint32_t)a};
+}
+struct DropCol { uint32_t hi, lo, c3; };
+__device__ __forceinline__ DropCol drop_col_part(const Drop& q, DropKey k, uint32_t group) {
+  const uint64_t a = (uint64_t)group * PHILOX_M0;
+  const uint64_t b = (uint64_t)((uint32_t)(a >> 32) ^ q.site ^ k.k1) * PHILOX_M1;
+  return DropCol{(uint32_t)(b >> 32), (uint32_t)b, (uint32_t)a};
+}
+__device__ __forceinline__ uint4 philox_rest(DropRow r, DropCol c, DropKey k) {
+  uint32_t c0 = c.hi ^ r.x, c1 = c.lo, c2 = r.hi ^ c.c3, c3 = r.lo;
+  k.k0 += 2u * PHILOX_W0; k.k1 += 2u * PHILOX_W1;
 #pragma unroll
-  for (int r = 0; r < 7; ++r) {
-    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+  for (int i = 2; i < 7; ++i) {
+    const uint64_t a = (uint64_t)c0 * PHILOX_M0, b = (uint64_t)c2 * PHILOX_M1;
     c0 = (uint32_t)(b >> 32) ^ c1 ^ k.k0; c1 = (uint32_t)b;
     c2 = (uint32_t)(a >> 32) ^ c3 ^ k.k1; c3 = (uint32_t)a;
-    k.k0 += 0x9E3779B9u; k.k1 += 0xBB67AE85u;
+    k.k0 += PHILOX_W0; k.k1 += PHILOX_W1;
   }
   return make_uint4(c0, c1, c2, c3);
 }
-// The eight columns of vector c of a row: v = v / (1 - p) or 0.  One rounding of the product, and none fused into what follows, as a
-// multiplication of its own has it; a dropped NaN or infinity is gone.
-__device__ __forceinline__ void drop8(const Drop& q, DropKey k, uint64_t row, int c, float (&v)[8]) {
-  const uint4 a = philox7(2u * c, (uint32_t)row, (uint32_t)(row >> 32), q.site, k);
-  const uint4 b = philox7(2u * c + 1u, (uint32_t)row, (uint32_t)(row >> 32), q.site, k);
+// Which of the eight columns of a vector are kept, a bit each.
+__device__ __forceinline__ uint32_t drop_bits(const Drop& q, DropKey k, DropRow r, DropCol c0, DropCol c1) {
+  const uint4 a = philox_rest(r, c0, k), b = philox_rest(r, c1, k);
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t bits = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = w[j] >= q.threshold ? __fmul_rn(v[j], q.scale) : 0.f;
+  for (int j = 0; j < 8; ++j) bits |= w[j] >= q.threshold ? 1u << j : 0u;
+  return bits;
+}
+// v = v / (1 - p) or 0.  One rounding of the product, and none fused into what follows, as a multiplication of its own has it; a dropped
+// NaN or infinity is gone.
+__device__ __forceinline__ void drop8(const Drop& q, uint32_t bits, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = bits >> j & 1u ? __fmul_rn(v[j], q.scale) : 0.f;
 }
 
-// y = drop(x); its own gradient, too.  Bound by memory: 2 bytes in and 2 out per element.
+// y = drop(x); its own gradient, too.  A thread takes one vector of four consecutive rows.  131072 x 2048 226 us, 4.75 TB/s; with every
+// product of every round taken anew 265.
+constexpr int DROP_ROWS = 4;
 __global__ void __launch_bounds__(256)
-dropout_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, unsigned nvec, unsigned total, Drop q) {
+dropout_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, unsigned nvec, unsigned rows, unsigned total, Drop q) {
   pdl_release();
   pdl_wait();
   const DropKey key = drop_key(q);
   for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
-    const unsigned row = i / nvec;
-    float v[8];
-    unpack8(x[i], v);
-    drop8(q, key, drop_row(q, row), (int)(i - row * nvec), v);
-    y[i] = pack8(v);
+    const unsigned group = i / nvec, c = i - group * nvec, row0 = group * DROP_ROWS;
+    const size_t at = (size_t)row0 * nvec + c;
+    uint4 u[DROP_ROWS];
+#pragma unroll
+    for (int r = 0; r < DROP_ROWS; ++r) if (row0 + r < rows) u[r] = x[at + (size_t)r * nvec];
+    const DropCol c0 = drop_col_part(q, key, 2 * c), c1 = drop_col_part(q, key, 2 * c + 1);
+#pragma unroll
+    for (int r = 0; r < DROP_ROWS; ++r) {
+      if (row0 + r >= rows) break;
+      const uint32_t bits = drop_bits(q, key, drop_row_part(q, key, row0 + r), c0, c1);
+      float v[8];
+      unpack8(u[r], v);
+      drop8(q, bits, v);
+      y[at + (size_t)r * nvec] = pack8(v);
+    }
   }
 }
 
@@ -103,8 +139,11 @@ dropout_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, unsigned nvec
 // One warp per row; d % 8 == 0; MAXV = max 16-byte vectors per lane (d <= 256*MAXV).
 // If `res` != null: x_new = x + res is written to `xout` and normalised; DROP: x_new = x + drop(res).
 // LAYER = true -> LayerNorm (mean/var, optional bias); false -> RMSNorm.
+// Wide rows leave registers for one block of eight warps per SM; with the generator in between that is too few, three of four warps are
+// better (131072 x 4096 875 and 762 us).
+constexpr int norm_fwd_warps(int maxv, bool drop) { return drop && maxv == 16 ? 4 : 8; }
 template <bool LAYER, int MAXV, bool DROP>
-__global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
+__global__ void __launch_bounds__(DROP && MAXV == 16 ? 128 : 256, DROP && MAXV == 16 ? 3 : 1) norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
                                 const float* __restrict__ w, const float* __restrict__ b,
                                 __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
                                 float* __restrict__ stats, int rows, int d, float eps, Drop q) {
@@ -127,9 +166,17 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
       if (rr) pr[i] = rr[c];
     }
   }
-  DropKey key{};
-  uint64_t place = 0;
-  if (DROP) { key = drop_key(q); place = drop_row(q, (unsigned)row); }
+  uint32_t bits[DROP ? (MAXV + 3) / 4 : 1];                        // eight for each vector, taken while the loads are on their way
+  if (DROP) {
+    const DropKey key = drop_key(q);
+    const DropRow place = drop_row_part(q, key, (unsigned)row);
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) {
+      const int c = lane + i * 32;
+      if (i % 4 == 0) bits[i / 4] = 0;
+      if (c < nvec) bits[i / 4] |= drop_bits(q, key, place, drop_col_part(q, key, 2 * c), drop_col_part(q, key, 2 * c + 1)) << (8 * (i % 4));
+    }
+  }
   float s = 0.f, ss = 0.f;
 #pragma unroll
   for (int i = 0; i < MAXV; ++i) {
@@ -140,7 +187,7 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
       if (rr) {
         float r8[8];
         unpack8(pr[i], r8);
-        if (DROP) drop8(q, key, place, c, r8);
+        if (DROP) drop8(q, bits[i / 4] >> (8 * (i % 4)), r8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fadd_rn(v[j], r8[j]);
         px[i] = pack8(v);
@@ -183,7 +230,10 @@ __global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_
 // One warp per row, with dw / db added to shared memory, spent its time in those additions (compare-and-swap loops).
 // Cold L2, one warp per row -> this, us: 32768 x 4096 757 -> 206 (5.2 TB/s); 131072 x 2048 732 -> 367 (5.9); 8192 x 2048
 // 71 -> 36; 8192 x 384 20.5 -> 16.4; layer norm 4096 x 768 20.5 -> 16.3, 4096 x 384 16.4 -> 12.3.
-// DROP: the gradient of the dropped branch, drop(dx), goes to `dbranch`.
+// DROP: the gradient of the dropped branch, drop(dx), goes to `dbranch`.  The generator takes a good part of the time between two turns' loads,
+// so the next turn's rows are copied to shared memory meanwhile, by the thread that will read them: no barrier, two turns in flight.
+// 131072 x 2048 517 us without these copies, 498 with them, 461 with two rows at a time instead of four (5.8 TB/s).
+constexpr int norm_bwd_rows(bool drop) { return drop ? 2 : 4; }
 template <bool LAYER, int G, bool DROP>
 __global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
 norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy,
@@ -192,7 +242,7 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
                 float* __restrict__ dw, float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
   pdl_release();
   pdl_wait();
-  constexpr int TB = G > 256 ? 512 : 256, NG = TB / G, W = G / 32, R = 4;
+  constexpr int TB = G > 256 ? 512 : 256, NG = TB / G, W = G / 32, R = norm_bwd_rows(DROP);
   __shared__ float4 red[2][NG][W][LAYER ? 2 : 1];            // per warp: four rows' sums; two buffers, one barrier per turn
   __shared__ float part[NG > 1 ? TB * 8 : 1];                // used only when a block holds several groups
   const int g = threadIdx.x / G, c = threadIdx.x % G, lane = threadIdx.x & 31, warp = c >> 5;
@@ -203,11 +253,49 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
   if (on) load8f(w, c, 1.f, wv);
   DropKey key{};
   if (DROP) key = drop_key(q);
+  extern __shared__ uint4 ahead[];                           // DROP: [2][x, dy, dres][R][TB]
+  float nmean[R], nrstd[R];
+  const auto fetch = [&](long row0, int stage) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      nmean[r] = nrstd[r] = 0.f;
+      if (row0 + r < rows) {
+        const size_t off = (size_t)(row0 + r) * d;
+        uint4* to = ahead + ((size_t)stage * 3 * R + r) * TB + threadIdx.x;
+        if (on) {
+          copy_ahead16(to, (const uint4*)(x + off) + c);
+          copy_ahead16(to + R * TB, (const uint4*)(dy + off) + c);
+          if (dres) copy_ahead16(to + 2 * R * TB, (const uint4*)(dres + off) + c);
+        }
+        if (LAYER) nmean[r] = stats[2 * (row0 + r)];
+        nrstd[r] = stats[2 * (row0 + r) + 1];
+      }
+    }
+    copy_ahead_commit();
+  };
+  const long step = (long)gridDim.x * NG * R;
+  if (DROP) fetch((long)blockIdx.x * NG * R + g * R, 0);
   int buf = 0;
-  for (long base = (long)blockIdx.x * NG * R; base < rows; base += (long)gridDim.x * NG * R, buf ^= 1) {
+  for (long base = (long)blockIdx.x * NG * R; base < rows; base += step, buf ^= 1) {
     const long row0 = base + g * R;
     uint4 px[R], pd[R], pr[R];
     float mean[R], rstd[R], s1[R], s2[R];
+    if (DROP) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) { mean[r] = nmean[r]; rstd[r] = nrstd[r]; }
+      fetch(row0 + step, buf ^ 1);
+      copy_ahead_wait1();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        px[r] = pd[r] = pr[r] = make_uint4(0, 0, 0, 0);
+        const uint4* at = ahead + ((size_t)buf * 3 * R + r) * TB + threadIdx.x;
+        if (on && row0 + r < rows) {
+          px[r] = at[0];
+          pd[r] = at[R * TB];
+          if (dres) pr[r] = at[2 * R * TB];
+        }
+      }
+    } else
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       px[r] = pd[r] = pr[r] = make_uint4(0, 0, 0, 0);
@@ -222,6 +310,12 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
         if (LAYER) mean[r] = stats[2 * (row0 + r)];
         rstd[r] = stats[2 * (row0 + r) + 1];
       }
+    }
+    uint32_t bits = 0;                                             // of the four rows, eight each
+    if (DROP && on) {
+      const DropCol c0 = drop_col_part(q, key, 2 * c), c1 = drop_col_part(q, key, 2 * c + 1);
+#pragma unroll
+      for (int r = 0; r < R; ++r) bits |= drop_bits(q, key, drop_row_part(q, key, (unsigned)(row0 + r)), c0, c1) << (8 * r);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -240,8 +334,8 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
     }
     if (W > 1) {
       if (lane == 0) {
-        red[buf][g][warp][0] = make_float4(s1[0], s1[1], s1[2], s1[3]);
-        if (LAYER) red[buf][g][warp][LAYER ? 1 : 0] = make_float4(s2[0], s2[1], s2[2], s2[3]);
+        red[buf][g][warp][0] = make_float4(s1[0], s1[1], s1[R - 2], s1[R - 1]);
+        if (LAYER) red[buf][g][warp][LAYER ? 1 : 0] = make_float4(s2[0], s2[1], s2[R - 2], s2[R - 1]);
       }
       __syncthreads();
 #pragma unroll
@@ -249,10 +343,12 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float4 v = red[buf][g][i][0];
-        s1[0] += v.x; s1[1] += v.y; s1[2] += v.z; s1[3] += v.w;
+        s1[0] += v.x; s1[1] += v.y;
+        if (R == 4) { s1[R - 2] += v.z; s1[R - 1] += v.w; }
         if (LAYER) {
           const float4 u = red[buf][g][i][LAYER ? 1 : 0];
-          s2[0] += u.x; s2[1] += u.y; s2[2] += u.z; s2[3] += u.w;
+          s2[0] += u.x; s2[1] += u.y;
+          if (R == 4) { s2[R - 2] += u.z; s2[R - 1] += u.w; }
         }
       }
     }
@@ -270,7 +366,7 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
       }
       ((uint4*)(dx + (size_t)(row0 + r) * d))[c] = pack8(o);
       if (DROP) {
-        drop8(q, key, drop_row(q, (unsigned)(row0 + r)), c, o);
+        drop8(q, bits >> (8 * r), o);
         ((uint4*)(dbranch + (size_t)(row0 + r) * d))[c] = pack8(o);
       }
     }
@@ -987,8 +1083,8 @@ extern "C" int cpb_dropout(const void* x, void* y, long rows, int d, const int64
   Drop q;
   const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
   if (rc != CPB_OK) return rc;
-  const unsigned total = (unsigned)(rows * (d / 8));
-  CPB_CUDA_OK(launch_pdl(dropout_kernel, grid_for(total, 256), 256, 0, stream, (const uint4*)x, (uint4*)y, (unsigned)d / 8, total, q));
+  const unsigned total = (unsigned)((rows + DROP_ROWS - 1) / DROP_ROWS * (d / 8));
+  CPB_CUDA_OK(launch_pdl(dropout_kernel, grid_for(total, 256), 256, 0, stream, (const uint4*)x, (uint4*)y, (unsigned)d / 8, (unsigned)rows, total, q));
   return check_launch("dropout");
 }
 
@@ -1007,7 +1103,7 @@ static int norm_fwd(const void* x, const void* res, const float* w, const float*
                     int layer, const Drop& q, cudaStream_t stream) {
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
-  const int wpb = 8;
+  const int wpb = norm_fwd_warps((d / 8 + 31) / 32 > 8 ? 16 : 8, q.seed != nullptr);
   decltype(&norm_fwd_kernel<true, 1, false>) kern;
   if (q.seed != nullptr) {
     if (layer) NORM_DISPATCH(norm_fwd_kernel, true, true);
@@ -1043,11 +1139,13 @@ static int norm_bwd(const void* x, const void* dy, const void* dres, const float
   if (nvec > 512) return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);
 #define NORM_BWD(G)                                                                                                             \
   do {                                                                                                                          \
-    const int tb = G > 256 ? 512 : 256, per_block = 4 * (tb / G);                                                               \
+    const int tb = G > 256 ? 512 : 256, R = norm_bwd_rows(q.seed != nullptr), per_block = R * (tb / G);                  \
     const int cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block, blocks = need < cap ? need : cap; \
     auto kern = q.seed != nullptr ? (layer ? norm_bwd_kernel<true, G, true> : norm_bwd_kernel<false, G, true>)                  \
                                   : (layer ? norm_bwd_kernel<true, G, false> : norm_bwd_kernel<false, G, false>);               \
-    CPB_CUDA_OK(launch_pdl(kern, blocks, tb, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats,    \
+    const size_t smem = q.seed != nullptr ? (size_t)2 * 3 * R * 16 * tb : 0;                                                    \
+    if (smem) CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                  \
+    CPB_CUDA_OK(launch_pdl(kern, blocks, tb, smem, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats,    \
                                     (__nv_bfloat16*)dx, dw, db, rows, d, (__nv_bfloat16*)dbranch, q));                           \
   } while (0)
   if (nvec <= 32) NORM_BWD(32);
