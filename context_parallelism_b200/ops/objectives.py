@@ -144,8 +144,8 @@ def _weights(w):
     return w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] and _rows16(w) else w.contiguous() if w.data_ptr() % 16 == 0 or not w.is_contiguous() else w.clone()
 
 
-def _backward(head, kept, w, h, each, g, want_dx, want_dw):
-    """``dx`` and ``dw`` (None where it went to ``main_grad``) from ``dloss / dlogp``."""
+def _backward(head, kept, w, h, each, most, g, want_dx, want_dw):
+    """``dx`` and ``dw`` (None where it went to ``main_grad``) from ``dloss / dlogp``, of which ``most`` is the address of the largest size, or 0."""
     dx = torch.empty(head.shape, dtype=torch.bfloat16, device=w.device) if want_dx else None
     mg = getattr(head.w, "main_grad", None) if want_dw else None
     own = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device) if want_dw and mg is None else None
@@ -157,7 +157,7 @@ def _backward(head, kept, w, h, each, g, want_dx, want_dw):
         wr = _weights(w)
         scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
         nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, kind, want_dx) - head.store - 1
-        nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, nv.ptr(g), nv.ptr(dx),
+        nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, most, nv.ptr(g), nv.ptr(dx),
                 (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.store, scratch.data_ptr(), head.chunk,
                 nv.status_for(w.device).ptr(), nv.stream_ptr(w.device))
     if mg is not None:
@@ -179,7 +179,7 @@ class _LogprobsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         w, kept = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, g.float().contiguous(), 1, None, *ctx.needs_input_grad[:2])
+        dx, dw = _backward(ctx.head, kept, w, g.float().contiguous(), 1, 0, None, *ctx.needs_input_grad[:2])
         return dx, dw, None, None
 
 
@@ -198,7 +198,7 @@ class _PolicyFn(torch.autograd.Function):
         if g is None:
             return None, None, None, None, None
         w, kept = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, None, 0, g.float().contiguous(), *ctx.needs_input_grad[:2])
+        dx, dw = _backward(ctx.head, kept, w, None, 0, 0, g.float().contiguous(), *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None
 
 
@@ -210,7 +210,7 @@ class _PreferenceFn(torch.autograd.Function):
         parts = max(1, -(-T // PART))
         sums = torch.empty((seqs, parts), dtype=torch.float64, device=x.device)
         loss = torch.empty((), dtype=torch.float32, device=x.device)
-        ratios, h = (torch.empty(seqs, dtype=torch.float32, device=x.device) for _ in range(2))
+        ratios, h = torch.empty(seqs, dtype=torch.float32, device=x.device), torch.empty(seqs + 1, dtype=torch.float32, device=x.device)
         stream = nv.stream_ptr(x.device)
         mine = (logp.data_ptr(), ref.data_ptr(), targets.data_ptr())
         if T == 0:
@@ -234,7 +234,7 @@ class _PreferenceFn(torch.autograd.Function):
         if g is None:
             return (None,) * 9
         w, kept, h = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, h, max(1, ctx.head.shape[1]), g.float().contiguous(), *ctx.needs_input_grad[:2])
+        dx, dw = _backward(ctx.head, kept, w, h, max(1, ctx.head.shape[1]), h[-1:].data_ptr(), g.float().contiguous(), *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None, None, None, None, None
 
 

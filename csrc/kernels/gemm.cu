@@ -492,7 +492,7 @@ using namespace cpb;
 // splits - 1 (bf16: splits) matrices of M x N floats, and a second launch adds them to C (bf16: sums them, adds the bias and rounds once).
 static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const float* bias,
                      int M, int N, int K, int lda, int ldb, int ldc, int ld_aux,
-                     int a_mn, int b_mn, int epi, float* partials, int splits, const Live& live, int* status, cudaStream_t stream) {
+                     int a_mn, int b_mn, int epi, float* partials, int splits, const float* factor, const Live& live, int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0) return set_error(CPB_ERR_ARG, "gemm: empty problem %dx%dx%d", M, N, K);
   // the contiguous dimension of every operand and every row stride must be a multiple of 8 elements (16 bytes)
   if ((N % 8) || (lda % 8) || (ldb % 8)) return set_error(CPB_ERR_ARG, "gemm: N,lda,ldb must be multiples of 8 (got N=%d lda=%d ldb=%d)", N, lda, ldb);
@@ -521,7 +521,7 @@ static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const flo
   p.band = tile_band(N, K);
   const int per_tile = epi == EPI_BF16_SWIGLU ? bn / 2 : bn;
   p.num_n_blocks = (N + per_tile - 1) / per_tile;
-  p.has_aux = aux != nullptr; p.bias = bias; p.status = status; p.live = live;
+  p.has_aux = aux != nullptr; p.bias = bias; p.status = status; p.factor = factor; p.live = live;
   const bool sum16 = splits > 1 && epi == EPI_BF16;      // every split goes to the workspace, the sum kernel writes C
   if (sum16) { p.epi = EPI_F32; p.bias = nullptr; }
 
@@ -564,7 +564,7 @@ static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const flo
 extern "C" int cpb_gemm_bf16(const void* A, const void* B, void* C, void* aux, const float* bias,
                              int M, int N, int K, int lda, int ldb, int ldc, int ld_aux,
                              int a_mn, int b_mn, int epi, float* partials, int splits, int* status, cudaStream_t stream) {
-  return gemm_bf16(A, B, C, aux, bias, M, N, K, lda, ldb, ldc, ld_aux, a_mn, b_mn, epi, partials, splits, Live{}, status, stream);
+  return gemm_bf16(A, B, C, aux, bias, M, N, K, lda, ldb, ldc, ld_aux, a_mn, b_mn, epi, partials, splits, nullptr, Live{}, status, stream);
 }
 
 static int gemm_head(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
@@ -617,14 +617,14 @@ extern "C" int cpb_gemm_head(const void* x, const void* w, void* out, const int6
 // The same two for objectives.cu, with rows counted on the device.
 namespace cpb {
 int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t stream) {
-  return gemm_bf16(g.A, g.B, g.C, nullptr, nullptr, g.M, g.N, g.K, g.lda, g.ldb, g.ldc, 0, g.a_mn, g.b_mn, g.epi, g.partials, g.splits, live, status, stream);
+  return gemm_bf16(g.A, g.B, g.C, nullptr, nullptr, g.M, g.N, g.K, g.lda, g.ldb, g.ldc, 0, g.a_mn, g.b_mn, g.epi, g.partials, g.splits, g.factor, live, status, stream);
 }
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream) {
   return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, head_parts(K) == 2, status, stream);
 }
-int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const Live& live, int* status,
-                    cudaStream_t stream) {
+int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const float* factor, const Live& live,
+                    int* status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0 || (N % 8) || (K % 8) || (ldw % 8) || most < 2) return set_error(CPB_ERR_ARG, "gemm_live_parts: %dx%dx%d in %d", M, N, K, most);
   GemmParams p{};
   p.M = M; p.N = N; p.K = K; p.epi = EPI_F32;
@@ -635,6 +635,7 @@ int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, in
   p.k_per_split = (p.num_k_blocks + most - 1) / most;
   p.band = tile_band(N, K);
   p.status = status;
+  p.factor = factor;
   p.live = live;
   CUtensorMap tm[4];
   int rc;

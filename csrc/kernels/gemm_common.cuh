@@ -62,6 +62,7 @@ struct GemmParams {
   int band;            // pair-rows per band of the tile order (1 = rows of tiles, columns fastest)
   int has_aux;
   const float* bias;
+  const float* factor;       // null, or one number in device memory that results of EPI_BF16, EPI_F32 and EPI_F32_ACC are multiplied with
   Live live;
   HeadParams head;
   int* status;
@@ -328,6 +329,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
                                               uint32_t t_row, int row0, int nb, int lane, int split, Release release) {
   const bool live = row0 < p.M;
   const float* bias = split == 0 ? p.bias : nullptr;
+  const float factor = p.factor != nullptr ? __ldg(p.factor) : 1.f;
   if (p.epi == EPI_BF16_SWIGLU) {
     // accumulator columns [0, BN/2) = gate, [BN/2, BN) = up, for features f0 .. f0 + BN/2
 #pragma unroll 1
@@ -364,6 +366,10 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
       tmem_wait_ld();
       if (c + 32 == BN) release();
       if (!live || col >= p.N) continue;
+      if (p.factor != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * factor);
+      }
       if (bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
@@ -405,6 +411,10 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
             }
           }
       }
+      if (p.factor != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) f[j] *= factor;
+      }
       uint32_t v[32];
       if (p.epi == EPI_BF16_GELU) {
         if (p.has_aux) {
@@ -431,13 +441,14 @@ struct GemmLive {
   const void *A, *B;
   void* C;
   int M, N, K, lda, ldb, ldc, a_mn, b_mn, epi;
+  const float* factor;       // see GemmParams
   float* partials;           // workspace of gemm_splits(M, N, K, epi) > 1: as many matrices of M x N floats (accumulating: one less)
   int splits;
 };
 // C fp32 [ranges][M][N], the partial products A w of as many ranges of K as *live.splits says, of at most `most`: A [M, K] and w [K, N]
 // row by row, tiles of `bn` columns.
-int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const Live& live, int* status,
-                    cudaStream_t stream);
+int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const float* factor, const Live& live,
+                    int* status, cudaStream_t stream);
 int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t stream);
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream);
