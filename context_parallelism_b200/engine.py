@@ -17,7 +17,7 @@ import torch.distributed as dist
 
 from . import graphs
 from .config import Config
-from .ops import permute
+from .ops import objectives, permute
 from .ops.optim import AdamW, FlatParams
 from .parallel.cp_attention import CPContext
 from .parallel.ddp import GradReducer
@@ -165,6 +165,75 @@ class TrainEngine:
         return self.model.graphs.run(f"micro-batch/{accum}", self.model, micro_batch,
                                      (tokens, targets, self.local_pos(tokens.shape[1]), *self.model.recorded_inputs()), self.device,
                                      graphs.model_flops(self.cfg, *tokens.shape, True), train=True)[0]
+
+    # ------------------------------------------------------------------ fine-tuning objectives
+    def _local_values(self, name: str, v, shape) -> Optional[torch.Tensor]:
+        """fp32 constants of an objective for the local tokens, of ``shape``: whole sequences are sharded as tokens are, local shards (as
+        ``token_logprobs`` returns them) and one value per sequence are taken as they are."""
+        if v is None:
+            return None
+        v = v.to(self.device, torch.float32, non_blocking=True)
+        if v.dim() == 1:
+            v = v[:, None]
+        B, T = shape
+        if v.dim() != 2 or v.shape[0] not in (1, B) or v.shape[1] not in (1, T, T * self.cp.cp_size):
+            raise ValueError(f"{name} of shape {tuple(v.shape)} for {B} sequences of {T * self.cp.cp_size} tokens ({T} here)")
+        if self.cp.cp_size > 1 and v.shape[1] == T * self.cp.cp_size:
+            v = permute.gather_seq(v.contiguous(), self.local_pos(T * self.cp.cp_size), 1)
+        return v
+
+    @torch.no_grad()
+    def token_logprobs(self, tokens, targets) -> torch.Tensor:
+        """Log-probabilities of the local tokens' targets (fp32 ``[B, T/cp]``, 0 where the target is negative), without gradients: what the
+        policy or a reference gives to the objectives below."""
+        idx, tgt, pos = self.shard_batch(tokens, targets)
+        return objectives.token_logprobs(self.model.hidden(idx, pos), self.model.head_weight(), tgt, self.cfg.vocab_size)
+
+    def _objective(self, tokens, targets, last: bool, scale: float, loss_of):
+        """Forward and backward pass of ``loss_of(hidden, head, local targets, targets)``, whose gradients count ``scale`` times."""
+        tokens, targets = self._taken(tokens), self._taken(targets)
+        self._next_dropout()
+        idx, tgt, pos = self.shard_batch(tokens, targets)
+        self.reducer.begin_backward()
+        with self.reducer.no_sync() if not last else _null():
+            out = loss_of(self.model.hidden(idx, pos), self.model.head_weight(), tgt,
+                          tgt if self.cp.cp_size == 1 else targets.to(self.device, non_blocking=True))
+            out.loss.backward(torch.full_like(out.loss, scale))
+        if last:
+            self.reducer.finish()
+        return out._replace(loss=out.loss.detach())
+
+    def policy_forward_backward(self, tokens, targets, old_logp, advantages, weights=None, ref_logp=None, clip=(0.2, 0.2), kl_coef: float = 0.0,
+                                accum: int = 1, last: bool = True) -> objectives.PolicyLoss:
+        """One micro-batch of ``objectives.linear_policy_loss`` in the place of ``forward_backward``; the update is ``optimizer_step``.
+
+        ``tokens`` and ``targets`` are whole sequences ``[B, T]`` as for a training step, targets negative where a token does not count.
+        Constants are ``[B, T]``, the local shards of ``token_logprobs``, or one value per sequence (``[B]``).  ``weights``: what a token
+        counts in the sum over the batch (None: the mean over its counted tokens).  Loss and terms are, averaged over the ranks as
+        ``global_loss`` does, those of the whole batch."""
+        def loss_of(h, w, tgt, whole):
+            wt = self._local_values("weights", weights, tgt.shape)
+            if wt is None:
+                wt = (1.0 / (whole >= 0).sum().clamp(min=1)).float().view(1, 1)
+            return objectives.linear_policy_loss(
+                h, w, tgt, self._local_values("old_logp", old_logp, tgt.shape), self._local_values("advantages", advantages, tgt.shape),
+                wt * self.cp.cp_size, self._local_values("ref_logp", ref_logp, tgt.shape), clip, kl_coef, self.cfg.vocab_size)
+        return self._objective(tokens, targets, last, 1.0 / accum, loss_of)
+
+    def preference_forward_backward(self, tokens, targets, ref_logp, weights=None, beta: float = 0.1, smoothing: float = 0.0, accum: int = 1,
+                                    last: bool = True) -> objectives.PreferenceLoss:
+        """One micro-batch of ``objectives.linear_preference_loss``: ``tokens`` ``[2 P, T]`` are the chosen answers, then the rejected ones in the
+        same order.  ``ref_logp`` as above.  ``weights`` ``[P]`` (None: the mean over the pairs).  The loss is that of the whole pairs on every
+        rank of a context-parallel group."""
+        def loss_of(h, w, tgt, whole):
+            pairs = tgt.shape[0] // 2
+            wt = torch.full((pairs,), 1.0 / max(1, pairs), device=self.device) if weights is None else weights.to(self.device, torch.float32, non_blocking=True)
+            group = None
+            if self.cp.cp_size > 1:
+                group = [self.cp.cp_group] if self.cp.cp_group is not None else [g for g in (self.cp.ring_group, self.cp.ulysses_group) if g is not None]
+            return objectives.linear_preference_loss(h, w, tgt, self._local_values("ref_logp", ref_logp, tgt.shape), wt, beta, smoothing,
+                                                     self.cfg.vocab_size, group)
+        return self._objective(tokens, targets, last, self.cp.cp_size / accum, loss_of)
 
     def optimizer_step(self) -> torch.Tensor:
         lr = self.lr_at(self.step_idx)

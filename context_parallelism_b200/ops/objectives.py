@@ -167,6 +167,12 @@ def _backward(head, kept, w, h, each, most, g, want_dx, want_dw):
     return dx, own
 
 
+def _sum_over(t, group):
+    for g in () if group is None else group if isinstance(group, (list, tuple)) else (group,):
+        dist.all_reduce(t, group=g)
+    return t
+
+
 # ----------------------------------------------------------------------------- autograd
 class _LogprobsFn(torch.autograd.Function):
     @staticmethod
@@ -219,8 +225,7 @@ class _PreferenceFn(torch.autograd.Function):
             nv.call("sequence_sums", *mine, sums.data_ptr(), seqs, T, parts, n_valid, stream)
         else:
             nv.LAUNCHES[0] += 1
-        if group is not None:
-            dist.all_reduce(sums, group=group)
+        _sum_over(sums, group)
         nv.call("preference", *(mine if T and group is None else (0, 0, 0)), T, n_valid, sums.data_ptr(), parts, seqs // 2, nv.ptr(weights), beta, smoothing,
                 loss.data_ptr(), ratios.data_ptr(), h.data_ptr(), stream)
         ctx.save_for_backward(w, kept, h)
@@ -277,8 +282,8 @@ def linear_preference_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tens
 
     ``ref_logp`` ``[2 P, T]``: log-probabilities of the same tokens under the reference policy, token by token, so that differences are summed
     and not the difference of two long sums taken.  ``weights`` (``[P]``, None: 1); a pair of weight 0 has no part in loss and gradient.
-    ``group``: the processes that hold shards of these sequences; ``R`` is summed over them, every rank returns the loss of the whole pairs
-    and the gradient of its own tokens."""
+    ``group``: the process group (or groups, one mesh axis each) that holds shards of these sequences; ``R`` is summed over it, every rank
+    returns the loss of the whole pairs and the gradient of its own tokens."""
     assert x.dim() == 3 and x.shape[0] % 2 == 0 and x.shape[0] > 0, f"hidden states of {tuple(x.shape)}: chosen answers, then as many rejected ones"
     targets, n_valid = _checked(x, w, targets, n_valid)
     ref = _per_token("ref_logp", ref_logp, targets)
@@ -321,9 +326,7 @@ class _SumOver(torch.autograd.Function):
     """Sum over the ranks of a group; every rank's gradient is that of its own part."""
     @staticmethod
     def forward(ctx, t, group):
-        t = t.clone()
-        dist.all_reduce(t, group=group)
-        return t
+        return _sum_over(t.clone(), group)
 
     @staticmethod
     def backward(ctx, g):

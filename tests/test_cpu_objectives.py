@@ -197,3 +197,61 @@ def test_plans():
     for bad in ((0, 8, 8, 256), (1, 0, 8, 256), (1, 8, 0, 256), (1, 8, 8, 0), (1, 8, 8, 100)):
         with pytest.raises(nv.NativeError):
             O._plan(*bad, False, 2, True)
+
+
+def _engine(**kw):
+    from context_parallelism_b200.config import Config
+    from context_parallelism_b200.engine import TrainEngine
+    cfg = Config.from_env("llama", 1, env={}).replace(**{**dict(n_embd=32, n_layer=1, n_head=2, n_kv_head=2, head_dim=16, ffn_hidden=64, vocab_size=50, T=8,
+                                                                B=4, dtype="fp32", checkpointing=False), **kw})
+    return TrainEngine(cfg, torch.device("cpu"))
+
+
+def _tokens(seed=0):
+    t = torch.randint(0, 50, (4, 9), generator=torch.Generator().manual_seed(seed))
+    x, y = t[:, :-1].contiguous(), t[:, 1:].contiguous()
+    y[0, :3], y[2, 6:] = -100, -1
+    return x, y
+
+
+def test_engine_means():
+    """Without weights a pass is the mean over counted tokens or pairs, and micro-batches add up to their mean."""
+    eng = _engine()
+    x, y = _tokens()
+    old = eng.token_logprobs(x, y)
+    n = int((y >= 0).sum())
+    adv = torch.tensor([1.0, -0.5, 0.25, 2.0])
+    out = eng.policy_forward_backward(x, y, old, adv, ref_logp=old - 0.2, kl_coef=0.5)
+    per = adv[:, None].expand(4, 8)[y >= 0]
+    assert float(out.loss) == pytest.approx(float(-per.mean() + 0.5 * (math.exp(-0.2) + 0.2 - 1)), rel=1e-5)
+    assert float(out.terms[3]) == pytest.approx(1.0, rel=1e-6)
+    one = eng.flat.grad.clone()
+    eng.opt.zero_grad()
+    for i in range(2):
+        eng.policy_forward_backward(x, y, old, adv, ref_logp=old - 0.2, kl_coef=0.5, accum=2, last=i == 1)
+    assert torch.allclose(eng.flat.grad, one, rtol=1e-5, atol=1e-8)
+    eng.opt.zero_grad()
+    wt = torch.full((4, 8), 1.0 / n)
+    eng.policy_forward_backward(x, y, old.double(), adv[:, None].expand(4, 8), weights=wt, ref_logp=old - 0.2, kl_coef=0.5)
+    assert torch.allclose(eng.flat.grad, one, rtol=1e-5, atol=1e-8)
+    eng.opt.zero_grad()
+    pref = eng.preference_forward_backward(x, y, old)
+    assert float(pref.loss) == pytest.approx(math.log(2), rel=1e-5) and pref.ratios.abs().max() < 1e-4
+    both = eng.flat.grad.clone()
+    eng.opt.zero_grad()
+    eng.preference_forward_backward(x, y, old, weights=torch.tensor([0.5, 0.5]))
+    assert torch.allclose(eng.flat.grad, both, rtol=1e-5, atol=1e-8)
+
+
+def test_engine_refuses():
+    eng = _engine()
+    x, y = _tokens()
+    z = torch.zeros(4, 8)
+    for bad in (torch.zeros(4, 7), torch.zeros(3, 8), torch.zeros(3), torch.zeros(4, 8, 1)):
+        for kw in (dict(old_logp=bad), dict(advantages=bad), dict(weights=bad), dict(ref_logp=bad)):
+            with pytest.raises(ValueError):
+                eng.policy_forward_backward(x, y, **{**dict(old_logp=z, advantages=z), **kw})
+        with pytest.raises(ValueError):
+            eng.preference_forward_backward(x, y, bad)
+    with pytest.raises(AssertionError):
+        eng.preference_forward_backward(x[:3], y[:3], z[:3])
