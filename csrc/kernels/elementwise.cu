@@ -139,14 +139,11 @@ dropout_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, unsigned nvec
 // One warp per row; d % 8 == 0; MAXV = max 16-byte vectors per lane (d <= 256*MAXV).
 // If `res` != null: x_new = x + res is written to `xout` and normalised; DROP: x_new = x + drop(res).
 // LAYER = true -> LayerNorm (mean/var, optional bias); false -> RMSNorm.
-// Wide rows leave registers for one block of eight warps per SM; with the generator in between that is too few, three of four warps are
-// better (131072 x 4096 875 and 762 us).
-constexpr int norm_fwd_warps(int maxv, bool drop) { return drop && maxv == 16 ? 4 : 8; }
 template <bool LAYER, int MAXV, bool DROP>
-__global__ void __launch_bounds__(DROP && MAXV == 16 ? 128 : 256, DROP && MAXV == 16 ? 3 : 1) norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
-                                const float* __restrict__ w, const float* __restrict__ b,
-                                __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
-                                float* __restrict__ stats, int rows, int d, float eps, Drop q) {
+__device__ __forceinline__ void norm_fwd_row(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
+                                             const float* __restrict__ w, const float* __restrict__ b,
+                                             __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
+                                             float* __restrict__ stats, int rows, int d, float eps, const Drop& q) {
   pdl_release();
   pdl_wait();
   const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -223,6 +220,24 @@ __global__ void __launch_bounds__(DROP && MAXV == 16 ? 128 : 256, DROP && MAXV =
   }
 }
 
+template <bool LAYER, int MAXV>
+__global__ void norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res,
+                                const float* __restrict__ w, const float* __restrict__ b,
+                                __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
+                                float* __restrict__ stats, int rows, int d, float eps) {
+  norm_fwd_row<LAYER, MAXV, false>(x, res, w, b, xout, y, stats, rows, d, eps, Drop{});
+}
+// Wide rows leave registers for one block of eight warps per SM; with the generator in between that is too few, three of four warps are
+// better (131072 x 4096 875 and 762 us).
+constexpr int norm_drop_warps(int maxv) { return maxv == 16 ? 4 : 8; }
+template <bool LAYER, int MAXV>
+__global__ void __launch_bounds__(32 * norm_drop_warps(MAXV), MAXV == 16 ? 3 : 1)
+norm_drop_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ res, const float* __restrict__ w,
+                     const float* __restrict__ b, __nv_bfloat16* __restrict__ xout, __nv_bfloat16* __restrict__ y,
+                     float* __restrict__ stats, int rows, int d, float eps, Drop q) {
+  norm_fwd_row<LAYER, MAXV, true>(x, res, w, b, xout, y, stats, rows, d, eps, q);
+}
+
 // ============================================================================ norm backward
 // dx = rstd * (g*dy - xhat * mean(g*dy*xhat) [- mean(g*dy)])  (+ dres_in) ; dw += sum dy*xhat ; db += sum dy
 // Bound by memory (x, dy, dres in, dx out).  A group of G threads owns the d columns, eight each, and takes four rows at a time:
@@ -233,16 +248,15 @@ __global__ void __launch_bounds__(DROP && MAXV == 16 ? 128 : 256, DROP && MAXV =
 // DROP: the gradient of the dropped branch, drop(dx), goes to `dbranch`.  The generator takes a good part of the time between two turns' loads,
 // so the next turn's rows are copied to shared memory meanwhile, by the thread that will read them: no barrier, two turns in flight.
 // 131072 x 2048 517 us without these copies, 498 with them, 461 with two rows at a time instead of four (5.8 TB/s).
-constexpr int norm_bwd_rows(bool drop) { return drop ? 2 : 4; }
+constexpr int norm_bwd_turn(bool drop) { return drop ? 2 : 4; }
 template <bool LAYER, int G, bool DROP>
-__global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
-norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy,
-                const __nv_bfloat16* __restrict__ dres, const float* __restrict__ w,
-                const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx,
-                float* __restrict__ dw, float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
+__device__ __forceinline__ void norm_bwd_rows(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy,
+                                              const __nv_bfloat16* __restrict__ dres, const float* __restrict__ w,
+                                              const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx, float* __restrict__ dw,
+                                              float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, const Drop& q) {
   pdl_release();
   pdl_wait();
-  constexpr int TB = G > 256 ? 512 : 256, NG = TB / G, W = G / 32, R = norm_bwd_rows(DROP);
+  constexpr int TB = G > 256 ? 512 : 256, NG = TB / G, W = G / 32, R = norm_bwd_turn(DROP);
   __shared__ float4 red[2][NG][W][LAYER ? 2 : 1];            // per warp: four rows' sums; two buffers, one barrier per turn
   __shared__ float part[NG > 1 ? TB * 8 : 1];                // used only when a block holds several groups
   const int g = threadIdx.x / G, c = threadIdx.x % G, lane = threadIdx.x & 31, warp = c >> 5;
@@ -401,6 +415,22 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
       }
     }
   }
+}
+
+template <bool LAYER, int G>
+__global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
+norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy,
+                const __nv_bfloat16* __restrict__ dres, const float* __restrict__ w,
+                const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx,
+                float* __restrict__ dw, float* __restrict__ db, int rows, int d) {
+  norm_bwd_rows<LAYER, G, false>(x, dy, dres, w, stats, dx, dw, db, rows, d, nullptr, Drop{});
+}
+template <bool LAYER, int G>
+__global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
+norm_drop_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ dres,
+                     const float* __restrict__ w, const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx, float* __restrict__ dw,
+                     float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
+  norm_bwd_rows<LAYER, G, true>(x, dy, dres, w, stats, dx, dw, db, rows, d, dbranch, q);
 }
 
 // ============================================================================ activations (backward)
@@ -1063,9 +1093,8 @@ static inline int grid_for(size_t work, int block, int per_sm = 8) {
 
 using namespace cpb;
 
-// The dropout of a launch; seed == null: none.
 static int make_drop(Drop& q, const int64_t* seed, const int64_t* pos, long rows, int T, long seq_len, long site, double p) {
-  if (seed == nullptr) { q = Drop{}; return CPB_OK; }
+  if (seed == nullptr) return set_error(CPB_ERR_ARG, "dropout: no seed");
   if (!(p >= 0. && p < 1.)) return set_error(CPB_ERR_ARG, "dropout: p=%g outside [0, 1)", p);
   if (T <= 0 || rows % T || rows > 0x7fffffffL || seq_len <= 0) return set_error(CPB_ERR_ARG, "dropout: %ld rows in sequences of %d of %ld", rows, T, seq_len);
   if (site < 0 || site > 0xffffffffL) return set_error(CPB_ERR_ARG, "dropout: site %ld outside 32 bits", site);
@@ -1078,8 +1107,8 @@ extern "C" int cpb_dropout(const void* x, void* y, long rows, int d, const int64
                            double p, cudaStream_t stream) {
   if (d <= 0 || d % 8) return set_error(CPB_ERR_ARG, "dropout: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
-  if (seed == nullptr || ((uintptr_t)x & 15) || ((uintptr_t)y & 15) || rows * (long)(d / 8) >= (1L << 31))
-    return set_error(CPB_ERR_ARG, "dropout: needs a seed, 16-byte aligned rows and less than 2^34 elements");
+  if (((uintptr_t)x & 15) || ((uintptr_t)y & 15) || rows * (long)(d / 8) >= (1L << 31))
+    return set_error(CPB_ERR_ARG, "dropout: needs 16-byte aligned rows and less than 2^34 elements");
   Drop q;
   const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
   if (rc != CPB_OK) return rc;
@@ -1088,89 +1117,100 @@ extern "C" int cpb_dropout(const void* x, void* y, long rows, int d, const int64
   return check_launch("dropout");
 }
 
-#define NORM_DISPATCH(KERN, LAYER, DROP)                                             \
+#define NORM_DISPATCH(KERN, LAYER)                                                   \
   do {                                                                               \
     const int nv = (d / 8 + 31) / 32;                                                \
-    if (nv <= 1) kern = KERN<LAYER, 1, DROP>;                                        \
-    else if (nv <= 2) kern = KERN<LAYER, 2, DROP>;                                   \
-    else if (nv <= 4) kern = KERN<LAYER, 4, DROP>;                                   \
-    else if (nv <= 8) kern = KERN<LAYER, 8, DROP>;                                   \
-    else if (nv <= 16) kern = KERN<LAYER, 16, DROP>;                                 \
+    if (nv <= 1) kern = KERN<LAYER, 1>;                                              \
+    else if (nv <= 2) kern = KERN<LAYER, 2>;                                         \
+    else if (nv <= 4) kern = KERN<LAYER, 4>;                                         \
+    else if (nv <= 8) kern = KERN<LAYER, 8>;                                         \
+    else if (nv <= 16) kern = KERN<LAYER, 16>;                                       \
     else return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);              \
   } while (0)
-
-static int norm_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y, float* stats, int rows, int d, float eps,
-                    int layer, const Drop& q, cudaStream_t stream) {
-  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
-  if (rows <= 0) return CPB_OK;
-  const int wpb = norm_fwd_warps((d / 8 + 31) / 32 > 8 ? 16 : 8, q.seed != nullptr);
-  decltype(&norm_fwd_kernel<true, 1, false>) kern;
-  if (q.seed != nullptr) {
-    if (layer) NORM_DISPATCH(norm_fwd_kernel, true, true);
-    else NORM_DISPATCH(norm_fwd_kernel, false, true);
-  } else {
-    if (layer) NORM_DISPATCH(norm_fwd_kernel, true, false);
-    else NORM_DISPATCH(norm_fwd_kernel, false, false);
-  }
-  CPB_CUDA_OK(launch_pdl(kern, (rows + wpb - 1) / wpb, wpb * 32, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)res, w, b, (__nv_bfloat16*)xout, (__nv_bfloat16*)y, stats, rows, d, eps, q));
-  return check_launch("norm_fwd");
-}
 
 // x (+res) -> xout (only when res != null), y ; stats [rows,2] (mean, rstd) optional
 extern "C" int cpb_norm_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y,
                             float* stats, int rows, int d, float eps, int layer, cudaStream_t stream) {
-  return norm_fwd(x, res, w, b, xout, y, stats, rows, d, eps, layer, Drop{}, stream);
+  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
+  if (rows <= 0) return CPB_OK;
+  const int wpb = 8;
+  decltype(&norm_fwd_kernel<true, 1>) kern;
+  if (layer) NORM_DISPATCH(norm_fwd_kernel, true);
+  else NORM_DISPATCH(norm_fwd_kernel, false);
+  CPB_CUDA_OK(launch_pdl(kern, (rows + wpb - 1) / wpb, wpb * 32, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)res, w, b, (__nv_bfloat16*)xout, (__nv_bfloat16*)y, stats, rows, d, eps));
+  return check_launch("norm_fwd");
 }
 
 // x + drop(res) -> xout, y
 extern "C" int cpb_norm_drop_fwd(const void* x, const void* res, const float* w, const float* b, void* xout, void* y, float* stats, int rows, int d,
                                  float eps, int layer, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site, double p, cudaStream_t stream) {
-  if (res == nullptr || seed == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs a residual branch and a seed");
+  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
+  if (rows <= 0) return CPB_OK;
   Drop q;
   const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
-  return rc != CPB_OK ? rc : norm_fwd(x, res, w, b, xout, y, stats, rows, d, eps, layer, q, stream);
+  if (rc != CPB_OK) return rc;
+  if (res == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs a residual branch");
+  const int wpb = norm_drop_warps(d > 2048 ? 16 : 8);
+  decltype(&norm_drop_fwd_kernel<true, 1>) kern;
+  if (layer) NORM_DISPATCH(norm_drop_fwd_kernel, true);
+  else NORM_DISPATCH(norm_drop_fwd_kernel, false);
+  CPB_CUDA_OK(launch_pdl(kern, (rows + wpb - 1) / wpb, wpb * 32, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)res, w, b, (__nv_bfloat16*)xout, (__nv_bfloat16*)y, stats, rows, d, eps, q));
+  return check_launch("norm_drop_fwd");
 }
 
-static int norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, float* dw, float* db, int rows,
-                    int d, int layer, void* dbranch, const Drop& q, cudaStream_t stream) {
+#define NORM_GROUPS(LAUNCH)         \
+  do {                              \
+    if (nvec <= 32) LAUNCH(32);     \
+    else if (nvec <= 64) LAUNCH(64);   \
+    else if (nvec <= 128) LAUNCH(128); \
+    else if (nvec <= 256) LAUNCH(256); \
+    else LAUNCH(512);               \
+  } while (0)
+
+// dw / db are fp32 and accumulated into (+=).
+extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats,
+                            void* dx, float* dw, float* db, int rows, int d, int layer, cudaStream_t stream) {
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
   const int nvec = d / 8;
   if (nvec > 512) return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);
 #define NORM_BWD(G)                                                                                                             \
   do {                                                                                                                          \
-    const int tb = G > 256 ? 512 : 256, R = norm_bwd_rows(q.seed != nullptr), per_block = R * (tb / G);                  \
+    const int tb = G > 256 ? 512 : 256, per_block = norm_bwd_turn(false) * (tb / G);                                            \
     const int cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block, blocks = need < cap ? need : cap; \
-    auto kern = q.seed != nullptr ? (layer ? norm_bwd_kernel<true, G, true> : norm_bwd_kernel<false, G, true>)                  \
-                                  : (layer ? norm_bwd_kernel<true, G, false> : norm_bwd_kernel<false, G, false>);               \
-    const size_t smem = q.seed != nullptr ? (size_t)2 * 3 * R * 16 * tb : 0;                                                    \
-    if (smem) CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                  \
-    CPB_CUDA_OK(launch_pdl(kern, blocks, tb, smem, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats,    \
-                                    (__nv_bfloat16*)dx, dw, db, rows, d, (__nv_bfloat16*)dbranch, q));                           \
+    auto kern = layer ? norm_bwd_kernel<true, G> : norm_bwd_kernel<false, G>;                                                   \
+    CPB_CUDA_OK(launch_pdl(kern, blocks, tb, 0, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats,    \
+                                    (__nv_bfloat16*)dx, dw, db, rows, d));                                                       \
   } while (0)
-  if (nvec <= 32) NORM_BWD(32);
-  else if (nvec <= 64) NORM_BWD(64);
-  else if (nvec <= 128) NORM_BWD(128);
-  else if (nvec <= 256) NORM_BWD(256);
-  else NORM_BWD(512);
+  NORM_GROUPS(NORM_BWD);
 #undef NORM_BWD
   return check_launch("norm_bwd");
-}
-
-// dw / db are fp32 and accumulated into (+=).
-extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats,
-                            void* dx, float* dw, float* db, int rows, int d, int layer, cudaStream_t stream) {
-  return norm_bwd(x, dy, dres, w, stats, dx, dw, db, rows, d, layer, nullptr, Drop{}, stream);
 }
 
 // as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped
 extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, void* dbranch,
                                  float* dw, float* db, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site,
                                  double p, cudaStream_t stream) {
-  if (dbranch == nullptr || seed == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs the branch's gradient and a seed");
+  if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
+  if (rows <= 0) return CPB_OK;
+  const int nvec = d / 8;
+  if (nvec > 512) return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);
   Drop q;
   const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
-  return rc != CPB_OK ? rc : norm_bwd(x, dy, dres, w, stats, dx, dw, db, rows, d, layer, dbranch, q, stream);
+  if (rc != CPB_OK) return rc;
+  if (dbranch == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs the branch's gradient");
+#define NORM_BWD(G)                                                                                                             \
+  do {                                                                                                                          \
+    const int tb = G > 256 ? 512 : 256, R = norm_bwd_turn(true), per_block = R * (tb / G), smem = 2 * 3 * R * 16 * tb;          \
+    const int cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block, blocks = need < cap ? need : cap; \
+    auto kern = layer ? norm_drop_bwd_kernel<true, G> : norm_drop_bwd_kernel<false, G>;                                         \
+    CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                 \
+    CPB_CUDA_OK(launch_pdl(kern, blocks, tb, smem, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats, \
+                                    (__nv_bfloat16*)dx, dw, db, rows, d, (__nv_bfloat16*)dbranch, q));                           \
+  } while (0)
+  NORM_GROUPS(NORM_BWD);
+#undef NORM_BWD
+  return check_launch("norm_drop_bwd");
 }
 
 extern "C" int cpb_swiglu_fwd(const void* gu, void* act, long rows, int F, cudaStream_t stream) {

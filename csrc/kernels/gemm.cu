@@ -116,7 +116,8 @@ __device__ __forceinline__ void pair_tile_coords(int tile, int num_m_tiles, int 
 }
 
 // EW epilogue warps: eight for the head's epilogues of shallow products (head_parts), two for each row, 128 columns each.
-template <int BN, bool A_MN, bool B_MN, int EW = 4>
+// LIVE: rows or K counted in device memory (Live), what the others are compiled without.
+template <int BN, bool A_MN, bool B_MN, bool LIVE, int EW = 4>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * EW, 1)
 gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmX, GemmParams p) {
@@ -136,6 +137,8 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const uint32_t rank = cluster_ctarank();      // 0: even CTA (issues the MMAs), 1: odd CTA
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
   int num_m_tiles = p.num_m_tiles, num_k_blocks = p.num_k_blocks, k_per_split = p.k_per_split, splits = p.splits;
+  int num_tiles = p.num_m_tiles * p.num_n_blocks;
+  int num_items = num_tiles * p.splits;         // item = split * num_tiles + tile: items of one K range run together
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -156,7 +159,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   if (p.splits == 1) pdl_release();
   pdl_wait();
   const uint32_t tmem_base = *tmem_slot;
-  if (p.live.count != nullptr) {
+  if (LIVE) {
     const int n = max(0, min(__ldg(p.live.count) - p.live.before, p.live.of_k ? p.K : p.M));
     if (p.live.of_k) {
       num_k_blocks = (n + GEMM_BK - 1) / GEMM_BK;
@@ -169,14 +172,14 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         k_per_split = (num_k_blocks + splits - 1) / splits;
       }
     }
+    num_tiles = num_m_tiles * p.num_n_blocks;
+    num_items = num_tiles * splits;
   }
-  const int num_tiles = num_m_tiles * p.num_n_blocks;
-  const int num_items = num_tiles * splits;     // item = split * num_tiles + tile: items of one K range run together
-  // the K blocks of a split; one that has none left takes the first block behind the operands, which TMA fills with zeros
+  // the K blocks of a split; with LIVE one that has none left takes the first block behind the operands, which TMA fills with zeros
   const auto k_range = [&](int split, int& kb0, int& kb1) {
     kb0 = split * k_per_split;
     kb1 = min(num_k_blocks, kb0 + k_per_split);
-    if (kb0 >= kb1) { kb0 = p.num_k_blocks; kb1 = kb0 + 1; }
+    if (LIVE && kb0 >= kb1) { kb0 = p.num_k_blocks; kb1 = kb0 + 1; }
   };
 
   if (warp == 0) {
@@ -285,7 +288,7 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       int mt, nb;
       pair_tile_coords(item % num_tiles, num_m_tiles, p.num_n_blocks, p.band, mt, nb);
       const int row0 = mt * (2 * GEMM_BM) + (int)rank * GEMM_BM + quarter * 32;
-      const HeadRow head = head_row(p, row0 + lane);
+      const HeadRow head = head_row<LIVE>(p, row0 + lane);
       bool ok = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, p.status, 310);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -299,10 +302,10 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           else mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
         }
       };
-      if (EW == 8) head_epilogue<BN / 2>(p, &tmC, ws, t_row + half * (BN / 2), row0, 2 * nb + half, lane, head, release);
-      else if (p.epi == EPI_HEAD_KEEP) head_keep_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
-      else if (p.epi >= EPI_HEAD_STATS) head_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
-      else gemm_epilogue<BN>(p, &tmC, &tmX, ws, t_row, row0, nb, lane, item / num_tiles, release);
+      if (EW == 8) head_epilogue<BN / 2, LIVE>(p, &tmC, ws, t_row + half * (BN / 2), row0, 2 * nb + half, lane, head, release);
+      else if (LIVE && p.epi == EPI_HEAD_KEEP) head_keep_epilogue<BN>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
+      else if (p.epi >= EPI_HEAD_STATS) head_epilogue<BN, LIVE>(p, &tmC, ws, t_row, row0, nb, lane, head, release);
+      else gemm_epilogue<BN, LIVE>(p, &tmC, &tmX, ws, t_row, row0, nb, lane, item / num_tiles, release);
     }
     ws.drain();
   }
@@ -316,9 +319,9 @@ gemm_pair_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
-template <int BN, bool A_MN, bool B_MN, int EW = 4>
+template <int BN, bool A_MN, bool B_MN, bool LIVE = false, int EW = 4>
 static int launch_pair(const CUtensorMap (&tm)[4], const GemmParams& p, cudaStream_t stream) {
-  auto kern = gemm_pair_bf16_kernel<BN, A_MN, B_MN, EW>;
+  auto kern = gemm_pair_bf16_kernel<BN, A_MN, B_MN, LIVE, EW>;
   static bool configured = false;
   if (!configured) {
     CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmSmem<BN, EW>::TOTAL));
@@ -502,6 +505,7 @@ static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const flo
   if (bias != nullptr && ((uintptr_t)bias & 15)) return set_error(CPB_ERR_ARG, "gemm: bias must be 16-byte aligned");
   if (epi != EPI_BF16_GELU && epi != EPI_BF16_SWIGLU) aux = nullptr;
   if (splits < 1) splits = 1;
+  if (live.count != nullptr && !(a_mn && b_mn && live.of_k)) return set_error(CPB_ERR_ARG, "gemm: a counted K is that of two operands stored along it");
   {
     const int nk = (K + GEMM_BK - 1) / GEMM_BK, kps = (nk + splits - 1) / splits;
     if (splits > 1 && ((epi != EPI_F32_ACC && epi != EPI_BF16) || partials == nullptr || ((uintptr_t)partials & 15) || (nk + kps - 1) / kps != splits))
@@ -552,7 +556,10 @@ static int gemm_bf16(const void* A, const void* B, void* C, void* aux, const flo
     uint32_t box[3] = {32, 32, 1};
     if ((rc = encode_tmap(&tm[3], partials, 4, 3, dims, strides, box, 1)) != CPB_OK) return rc;
   }
-  rc = bn == 384 ? dispatch_pair<384>(tm, p, a_mn, b_mn, stream) : bn == 256 ? dispatch_pair<256>(tm, p, a_mn, b_mn, stream) : bn == 192 ? dispatch_pair<192>(tm, p, a_mn, b_mn, stream) : dispatch_pair<128>(tm, p, a_mn, b_mn, stream);
+  if (live.count != nullptr)
+    rc = bn == 384 ? launch_pair<384, true, true, true>(tm, p, stream) : bn == 256 ? launch_pair<256, true, true, true>(tm, p, stream)
+         : bn == 192 ? launch_pair<192, true, true, true>(tm, p, stream) : launch_pair<128, true, true, true>(tm, p, stream);
+  else rc = bn == 384 ? dispatch_pair<384>(tm, p, a_mn, b_mn, stream) : bn == 256 ? dispatch_pair<256>(tm, p, a_mn, b_mn, stream) : bn == 192 ? dispatch_pair<192>(tm, p, a_mn, b_mn, stream) : dispatch_pair<128>(tm, p, a_mn, b_mn, stream);
   if (rc != CPB_OK || splits == 1) return rc;
   const unsigned total = (unsigned)((long)M * N / (sum16 ? 8 : 4)), blocks = (total + 255) / 256, cap = (unsigned)sm_count() * 8;
   const unsigned grid = blocks < cap ? blocks : cap;
@@ -598,7 +605,8 @@ static int gemm_head(const void* x, const void* w, void* out, int M, int N, int 
     if ((rc = encode_tmap(&tm[2], out, eb, 2, dims, strides, box, 1)) != CPB_OK) return rc;
   }
   tm[3] = tm[2];
-  return eight ? launch_pair<256, false, false, 8>(tm, p, stream) : launch_pair<256, false, false>(tm, p, stream);
+  if (live.count == nullptr) return launch_pair<256, false, false>(tm, p, stream);
+  return eight ? launch_pair<256, false, false, true, 8>(tm, p, stream) : launch_pair<256, false, false, true>(tm, p, stream);
 }
 
 // Cross entropy of the language-model head, logits = x w^T (x [M,K], w [N,K], both K-major).  out == null or fp32 (grad == 0): per row and
@@ -645,7 +653,8 @@ int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, in
   uint32_t box[3] = {32, 32, 1};
   if ((rc = encode_tmap(&tm[3], parts, 4, 3, dims, strides, box, 1)) != CPB_OK) return rc;
   tm[2] = tm[3];
-  return bn == 256 ? launch_pair<256, false, true>(tm, p, stream) : bn == 192 ? launch_pair<192, false, true>(tm, p, stream) : launch_pair<128, false, true>(tm, p, stream);
+  return bn == 256 ? launch_pair<256, false, true, true>(tm, p, stream) : bn == 192 ? launch_pair<192, false, true, true>(tm, p, stream)
+         : launch_pair<128, false, true, true>(tm, p, stream);
 }
 int gemm_splits(int M, int N, int K, int epi) {
   int bn = 256, splits = 1;

@@ -149,13 +149,14 @@ struct HeadRow {
   float scale;               // of the target's one
   bool off;                  // a row of zeros
 };
+template <bool LIVE>
 __device__ __forceinline__ HeadRow head_row(const GemmParams& p, int row) {
   HeadRow h{-1, {0.f, 0.f}, p.head.grad_scale, false};
   if (p.epi >= EPI_HEAD_STATS && row < p.M) {
     const int64_t t = __ldg(p.head.targets + row);
     h.target = t >= 0 && t < p.head.n_valid ? (int)t : -1;
     if (p.epi == EPI_HEAD_GRAD) h.coef = __ldg(p.head.row_coef + row);
-    if (p.head.row_scale != nullptr) {
+    if (LIVE && p.head.row_scale != nullptr) {
       h.scale = __ldg(p.head.row_scale + row);
       h.coef.y *= h.scale;
       h.off = h.scale == 0.f;
@@ -237,11 +238,12 @@ __device__ __forceinline__ void head_keep_epilogue(const GemmParams& p, const CU
 
 // Bound by the main loop from a K of about 300 on: a tile's 256 exponentials per thread take the special-function unit 2048 cycles,
 // 64 of K take 370 ns.
-template <int COLS, class Release>
+template <int COLS, bool LIVE, class Release>
 __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtensorMap* tmC, WarpStore& ws, uint32_t t_row, int row0, int part,
                                               int lane, const HeadRow& h, Release release) {
   const int row = row0 + lane;
   const bool live = row0 < p.M;
+  const float l2e1 = LIVE ? p.head.l2e : LOG2E;
   float m = -INFINITY, s = 0.f;
 #pragma unroll 1
   for (int c = 0; c < COLS; c += 64) {
@@ -277,10 +279,10 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
         for (int j = 8; j < 64; j += 8) mx[q] = fmax3(mx[q], f[j + q], f[j + q + 4]);
       }
       const float mt = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
-      if (mt > m) { s = m == -INFINITY ? s : s * ex2f((m - mt) * p.head.l2e); m = mt; }
+      if (mt > m) { s = m == -INFINITY ? s : s * ex2f((m - mt) * l2e1); m = mt; }
       // a row of nothing but -inf so far adds nothing; NaN gets into the sum, whatever the maximum says
       const float ref = m == -INFINITY ? 0.f : m;
-      const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
+      const uint64_t nm = pack_f32x2(-ref, -ref), l2e = pack_f32x2(l2e1, l2e1);
       uint64_t acc[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {
@@ -292,7 +294,7 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
       unpack_f32x2(add_f32x2(acc[0], acc[1]), a, b);
       s += a + b;
     } else {
-      const uint64_t nm = pack_f32x2(-h.coef.x, -h.coef.x), l2e = pack_f32x2(p.head.l2e, p.head.l2e);
+      const uint64_t nm = pack_f32x2(-h.coef.x, -h.coef.x), l2e = pack_f32x2(l2e1, l2e1);
       const uint64_t inv = pack_f32x2(h.coef.y, h.coef.y);
 #pragma unroll
       for (int j = 0; j < 64; j += 2) {
@@ -306,9 +308,9 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
       }
       if (hit) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) f[j] = j == at ? f[j] - h.scale : f[j];
+        for (int j = 0; j < 64; ++j) f[j] = j == at ? f[j] - (LIVE ? h.scale : p.head.grad_scale) : f[j];
       }
-      if (h.off) {
+      if (LIVE && h.off) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) f[j] = 0.f;
       }
@@ -324,12 +326,12 @@ __device__ __forceinline__ void head_epilogue(const GemmParams& p, const CUtenso
 // Epilogue of one 32-row slice of a 128 x BN accumulator tile: `t_row` is the tensor-memory address of this warp's lanes at
 // the accumulator's first column, `row0` the slice's first output row, `nb` the tile's index along N, `split` its range of K (the
 // first one brings the bias).  `release` runs as soon as the accumulator has been read.
-template <int BN, class Release>
+template <int BN, bool LIVE, class Release>
 __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtensorMap* tmC, const CUtensorMap* tmX, WarpStore& ws,
                                               uint32_t t_row, int row0, int nb, int lane, int split, Release release) {
   const bool live = row0 < p.M;
   const float* bias = split == 0 ? p.bias : nullptr;
-  const float factor = p.factor != nullptr ? __ldg(p.factor) : 1.f;
+  const float factor = LIVE && p.factor != nullptr ? __ldg(p.factor) : 1.f;
   if (p.epi == EPI_BF16_SWIGLU) {
     // accumulator columns [0, BN/2) = gate, [BN/2, BN) = up, for features f0 .. f0 + BN/2
 #pragma unroll 1
@@ -366,7 +368,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
       tmem_wait_ld();
       if (c + 32 == BN) release();
       if (!live || col >= p.N) continue;
-      if (p.factor != nullptr) {
+      if (LIVE && p.factor != nullptr) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * factor);
       }
@@ -411,7 +413,7 @@ __device__ __forceinline__ void gemm_epilogue(const GemmParams& p, const CUtenso
             }
           }
       }
-      if (p.factor != nullptr) {
+      if (LIVE && p.factor != nullptr) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) f[j] *= factor;
       }
