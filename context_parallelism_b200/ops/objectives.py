@@ -28,6 +28,7 @@ CHUNK_BYTES = 2 << 30            # of bf16 dlogits, the rows that go through the
 KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward to the backward pass
 # Width of the hidden states above which that is faster than to compute them again (and the head's GEMM has an epilogue that does).
 KEEP_ABOVE = 512
+FEW_ROWS = 256                   # up to which dlogits are the sum of two bf16 numbers
 PART = 4096                      # tokens of a sequence that one block adds up
 COUNT_ROWS = 4096                # up to which rows are counted and gathered in one launch
 
@@ -74,17 +75,17 @@ def _per_token(name, t, like, optional=False):
 
 # ----------------------------------------------------------------------------- launches
 @functools.lru_cache(maxsize=4096)
-def _plan(N: int, d: int, V: int, chunk: int, store: bool, dw: int, want_dx: bool) -> Tuple[int, int]:
+def _plan(N: int, d: int, V: int, chunk: int, keep: int, dw: int, want_dx: bool) -> Tuple[int, int]:
     out = (ctypes.c_int64 * 2)()
-    nv.check(nv.lib().cpb_objective_plan(N, d, V, chunk, store, dw, want_dx, ctypes.addressof(out)), "objective_plan")
+    nv.check(nv.lib().cpb_objective_plan(N, d, V, chunk, keep, dw, want_dx, ctypes.addressof(out)), "objective_plan")
     return tuple(out)
 
 
 @functools.lru_cache(maxsize=4096)
-def _backward_launches(N: int, d: int, V: int, chunk: int, dw: int, want_dx: bool) -> int:
-    n = 1 + (dw == 2 and N > chunk)
+def _backward_launches(N: int, d: int, V: int, chunk: int, keep: int, dw: int, want_dx: bool) -> int:
+    n = (keep == 0) + (dw == 2 and N > chunk)
     for r0 in range(0, N, chunk):
-        rows = min(chunk, N - r0)
+        rows = min(chunk, N - r0) if keep < 2 else 2 * (-(-N // 64) * 64)
         n += 1 + 2 * want_dx
         if dw:
             epi = EPI_BF16 if dw == 2 and N <= chunk else EPI_F32_ACC
@@ -108,7 +109,8 @@ class _Head:
         self.shape, self.w, self.n_valid, self.grad = x.shape, w, n_valid, grad
         self.N, self.d, self.V = targets.numel(), x.shape[-1], w.shape[0]
         self.chunk = _chunk(self.V)
-        self.store = grad and self.d > KEEP_ABOVE and 2 * self.N * self.V <= KEEP_BYTES
+        # 0 nothing, 1 the logits, 2 those of few rows
+        self.keep = 0 if not grad or 2 * self.N * self.V > KEEP_BYTES else 2 if self.N <= FEW_ROWS else int(self.d > KEEP_ABOVE)
 
 
 def _rows16(t):
@@ -131,12 +133,12 @@ def _forward(x, w, targets, n_valid, grad, policy=None):
     else:
         T, sb, st = head.N, 0, xr.stride(-2)
     wr = _weights(w)
-    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, 0, False)[0], dtype=torch.uint8, device=x.device)
+    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, 0, False)[0], dtype=torch.uint8, device=x.device)
     old, adv, weights, ref, low, high, kl = policy or (None, None, None, None, 0.0, 0.0, 0.0)
     chunks = -(-head.N // head.chunk)
     nv.LAUNCHES[0] += (head.N > COUNT_ROWS) + 2 * chunks
     nv.call("objective_fwd", xr.data_ptr(), sb, st, head.N, T, head.d, wr.data_ptr(), wr.stride(0), head.V, n_valid, targets.data_ptr(), nv.ptr(old),
-            nv.ptr(adv), nv.ptr(weights), nv.ptr(ref), low, high, kl, logp.data_ptr(), nv.ptr(loss), nv.ptr(terms), kept.data_ptr(), head.store, head.chunk, nv.status_for(x.device).ptr(), nv.stream_ptr(x.device))
+            nv.ptr(adv), nv.ptr(weights), nv.ptr(ref), low, high, kl, logp.data_ptr(), nv.ptr(loss), nv.ptr(terms), kept.data_ptr(), head.keep, head.chunk, nv.status_for(x.device).ptr(), nv.stream_ptr(x.device))
     return head, kept, logp, loss, terms
 
 
@@ -155,10 +157,10 @@ def _backward(head, kept, w, h, each, most, g, want_dx, want_dw):
             own.zero_()
     elif want_dx or want_dw:
         wr = _weights(w)
-        scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.store, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
-        nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, kind, want_dx) - head.store - 1
+        scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
+        nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, head.keep, kind, want_dx) - 1
         nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, most, nv.ptr(g), nv.ptr(dx),
-                (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.store, scratch.data_ptr(), head.chunk,
+                (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.keep, scratch.data_ptr(), head.chunk,
                 nv.status_for(w.device).ptr(), nv.stream_ptr(w.device))
     if mg is not None:
         hook = getattr(head.w, "_grad_ready", None)

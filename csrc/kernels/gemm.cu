@@ -629,7 +629,7 @@ int gemm_live(const GemmLive& g, const Live& live, int* status, cudaStream_t str
 }
 int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K, int ldx, int ldw, long ldc, int grad, const HeadParams& head,
                    const Live& live, int* status, cudaStream_t stream) {
-  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, head_parts(K) == 2, status, stream);
+  return gemm_head(x, w, out, M, N, K, ldx, ldw, ldc, grad, head, live, grad != 2 && head_parts(K) == 2, status, stream);
 }
 int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const float* factor, const Live& live,
                     int* status, cudaStream_t stream) {

@@ -17,7 +17,8 @@
 namespace cpb {
 
 struct Rows {                // the gathered rows, kept from the forward pass to the backward pass
-  int* live;                 // [0] how many, [1] a ticket
+  int* live;                 // [0] how many, [1] a ticket, [2] 2 x half
+  int half;                  // see FEW_ROWS; 0 where there are more
   int* ranges;               // [chunks] into how many ranges of K the product for dx is split
   int* from;                 // [N] gathered row -> row
   int* place;                // [N] row -> gathered row, or -1
@@ -25,10 +26,19 @@ struct Rows {                // the gathered rows, kept from the forward pass to
   float2* norm;              // [N] gathered: (max, 1 / sum of exponentials)
   float* h;                  // [N] gathered: dloss / dlogp, written by the policy loss
   float* target_p;           // [N] gathered: the target's probability
-  __nv_bfloat16* x;          // [N, d] gathered, zero from the last row to the next multiple of 64
+  __nv_bfloat16* x;          // [N, d] gathered, zero from the last row to the next multiple of 64; [2 x half, d] twice, zero to `half`
   float2* stats;             // [chunks][parts][rows of the chunk] (max, sum of exponentials), or null
   __half* logits;            // [N, V] gathered: distances to the part's max, or null
 };
+
+// Up to FEW_ROWS rows the products of the backward pass wait for the weights, not for the tensor core, and dlogits are given to them as a sum of
+// two bf16 numbers: `half` rows of rounded ones, and behind them as many of what the rounding has left, to which the gathered rows of x
+// stand a second time.  So the gradients of a short call, where no average over many rows makes up for it, are rounded once.  Error of dx and
+// dw against 64 bits over that of results rounded once: 136 rows 1.3 to 1.5, now 1.00.
+// keep: 0 logits are computed again, 1 kept, 2 kept and dlogits in two parts.
+constexpr int FEW_ROWS = 256;
+enum : int { KEEP_NONE = 0, KEEP_LOGITS = 1, KEEP_FEW = 2 };
+static int half_rows(long N, int keep) { return keep == KEEP_FEW ? (int)((N + 63) / 64 * 64) : 0; }
 
 __device__ __forceinline__ bool row_counts(const int64_t* targets, const float* weights, int row, int n_valid) {
   const int64_t t = targets[row];
@@ -116,9 +126,9 @@ rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T,
     if (lane == 0) { s_base = base; s_n = __popc(mask); }
     if (group == (int)gridDim.x - 1) {
       const int live = base + __popc(mask);
-      if (lane == 0) { r.live[0] = live; if (COUNT) r.live[1] = 0; }
+      if (lane == 0) { r.live[0] = live; r.live[2] = 2 * r.half; if (COUNT) r.live[1] = 0; }
       for (int c = 0; c * chunk < N; ++c) {
-        const int s = ranges_of(q, max(0, min(chunk, live - c * chunk)));
+        const int s = ranges_of(q, r.half ? 2 * r.half : max(0, min(chunk, live - c * chunk)));
         if (lane == 0) r.ranges[c] = s;
       }
     }
@@ -134,13 +144,20 @@ rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T,
 #pragma unroll
       for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) v[k] = src[c + 32 * k];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) if (c + 32 * k < nvec) dst[c + 32 * k] = v[k];
+      for (int k = 0; k < 4; ++k) {
+        if (c + 32 * k >= nvec) continue;
+        dst[c + 32 * k] = v[k];
+        if (r.half) dst[(size_t)r.half * nvec + c + 32 * k] = v[k];
+      }
     }
   }
   if (group == (int)gridDim.x - 1) {                               // K of the weight gradient is taken 64 rows at a time
-    const int total = s_base + s_n, end = min(N, (total + 63) & ~63);
+    const int total = s_base + s_n, end = r.half ? r.half : min(N, (total + 63) & ~63);
     for (int i = total + warp; i < end; i += 8)
-      for (int c = lane; c < nvec; c += 32) ((uint4*)(r.x + (size_t)i * d))[c] = make_uint4(0, 0, 0, 0);
+      for (int c = lane; c < nvec; c += 32) {
+        ((uint4*)(r.x + (size_t)i * d))[c] = make_uint4(0, 0, 0, 0);
+        if (r.half) ((uint4*)(r.x + (size_t)(r.half + i) * d))[c] = make_uint4(0, 0, 0, 0);
+      }
   }
 }
 
@@ -359,7 +376,7 @@ rows_dlogits_kernel(Rows r, const float* __restrict__ h, int each, const float* 
   float back;
   const float factor = even_factor(even, g, back);
   if (at == 0 && blockIdx.x == 0 && threadIdx.x == 0) *even.back = back;
-  if (at >= ((live + 63) & ~63)) return;
+  if (at >= (r.half ? r.half : (live + 63) & ~63)) return;
   const float s = at < live ? row_scale(r, h, each, g, at) * factor : 0.f;
   const bool on = s != 0.f;                                        // a row of gradient 0 is zero, whatever its logits are
   const int c0 = blockIdx.x * RD_COLS + 8 * threadIdx.x;
@@ -401,7 +418,14 @@ rows_dlogits_kernel(Rows r, const float* __restrict__ h, int each, const float* 
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = tgt == c + e ? one : p[e];
     }
-    *(uint4*)(dlogits + (size_t)row * V + c) = make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7]));
+    const uint4 out = make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7]));
+    *(uint4*)(dlogits + (size_t)row * V + c) = out;
+    if (r.half) {
+      const uint32_t o[4] = {out.x, out.y, out.z, out.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { p[2 * e] -= bf16_lo(o[e]); p[2 * e + 1] -= bf16_hi(o[e]); }
+      *(uint4*)(dlogits + (size_t)(r.half + row) * V + c) = make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7]));
+    }
   }
 }
 
@@ -409,7 +433,7 @@ rows_dlogits_kernel(Rows r, const float* __restrict__ h, int each, const float* 
 // Eight columns per thread, bound by the parts' way through L2.
 __global__ void __launch_bounds__(256)
 rows_scatter_kernel(const float* __restrict__ parts, const int* __restrict__ ranges, const int* __restrict__ place, __nv_bfloat16* __restrict__ out,
-                    int N, int d, int before, int rows, size_t total) {
+                    int N, int d, int before, int rows, int half, size_t total) {
   pdl_release();
   pdl_wait();
   const int count = *ranges, nvec = d >> 3;
@@ -421,6 +445,14 @@ rows_scatter_kernel(const float* __restrict__ parts, const int* __restrict__ ran
     if (to >= 0) {
       const float4* src = (const float4*)(parts + (size_t)at * d) + 2 * c;
       a = src[0]; b = src[1];
+      if (half) {
+        const float4* low = src + (size_t)half * d / 4;
+        for (int s = 0; s < count; ++s) {
+          const float4 u = low[s * step], v = low[s * step + 1];
+          a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+          b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+        }
+      }
       int s = 1;
       for (; s + 3 < count; s += 4) {
         float4 u[4], v[4];
@@ -467,9 +499,10 @@ static size_t take(size_t& at, size_t bytes) {
   return here;
 }
 // `base` may be null: the size alone
-static Rows rows_layout(char* base, long N, int d, long V, int chunk, int store, size_t& bytes) {
+static Rows rows_layout(char* base, long N, int d, long V, int chunk, int keep, size_t& bytes) {
   size_t at = 0;
   Rows r;
+  r.half = half_rows(N, keep);
   r.live = (int*)(base + take(at, 256));
   r.ranges = (int*)(base + take(at, (N / chunk + 1) * 4));
   r.from = (int*)(base + take(at, N * 4));
@@ -478,20 +511,20 @@ static Rows rows_layout(char* base, long N, int d, long V, int chunk, int store,
   r.norm = (float2*)(base + take(at, N * 8));
   r.h = (float*)(base + take(at, N * 4));
   r.target_p = (float*)(base + take(at, N * 4));
-  r.x = (__nv_bfloat16*)(base + take(at, (size_t)N * d * 2));
-  r.stats = store ? (float2*)(base + take(at, (size_t)((V + 255) / 256) * N * 8)) : nullptr;
-  r.logits = store ? (__half*)(base + take(at, (size_t)N * V * 2)) : nullptr;
+  r.x = (__nv_bfloat16*)(base + take(at, (size_t)(r.half ? 2 * r.half : N) * d * 2));
+  r.stats = keep ? (float2*)(base + take(at, (size_t)((V + 255) / 256) * N * 8)) : nullptr;
+  r.logits = keep ? (__half*)(base + take(at, (size_t)N * V * 2)) : nullptr;
   bytes = at;
   return r;
 }
 // What the forward pass alone needs stands behind the rows, in the same buffer: it is small, and an allocation costs the host 3 us.
 struct FwdScratch { int* counts; float2* stats; float* target_logit; double* part; };
-static FwdScratch fwd_layout(char* base, long N, int d, long V, int chunk, int store, size_t& bytes) {
+static FwdScratch fwd_layout(char* base, long N, int d, long V, int chunk, int keep, size_t& bytes) {
   size_t at = bytes;
   const long rows = N < chunk ? N : chunk, parts = (V + 255) / 256 * head_parts(d);
   FwdScratch s;
   s.counts = (int*)(base + take(at, (N + 31) / 32 * 4));
-  s.stats = (float2*)(base + take(at, store ? 0 : (size_t)parts * rows * 8));
+  s.stats = (float2*)(base + take(at, keep ? 0 : (size_t)parts * rows * 8));
   s.target_logit = (float*)(base + take(at, rows * 4));
   s.part = (double*)(base + take(at, ((N + 31) / 32 + N / chunk + 1) * 32));
   bytes = at;
@@ -515,9 +548,10 @@ static Ranges dx_ranges(int rows, int d, int V) {
   return q;
 }
 struct BwdScratch { float *scale, *back; __nv_bfloat16* dlogits; float *dx, *dw, *partials; };
-static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int dw, int want_dx, size_t& bytes) {
+static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int keep, int dw, int want_dx, size_t& bytes) {
   size_t at = 0;
-  const long rows = N < chunk ? N : chunk;
+  const int half = half_rows(N, keep);
+  const long rows = half ? 2 * half : N < chunk ? N : chunk;
   const bool one = N <= chunk;
   BwdScratch s;
   s.scale = (float*)(base + take(at, N * 4));
@@ -526,7 +560,7 @@ static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int d
   s.dw = (float*)(base + take(at, dw == DW_BF16 && !one ? (size_t)V * d * 4 : 0));
   size_t parts = 0, most = 0;
   for (long r0 = 0; r0 < N; r0 += chunk) {                         // the last chunk has a plan of its own
-    const long n = N - r0 < chunk ? N - r0 : chunk;
+    const long n = half ? 2 * half : N - r0 < chunk ? N - r0 : chunk;
     if (r0 > 0 && n == chunk) continue;
     if (want_dx) {
       const size_t m = (size_t)dx_ranges((int)n, d, (int)V).most * n * d;
@@ -549,17 +583,19 @@ static BwdScratch bwd_layout(char* base, long N, int d, long V, int chunk, int d
 using namespace cpb;
 
 // Bytes of the buffers of an objective over N rows of width d and V columns: kept between the passes, and of the backward pass.
-extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int store, int dw, int want_dx, int64_t* bytes) {
+extern "C" int cpb_objective_plan(int N, int d, int V, int chunk, int keep, int dw, int want_dx, int64_t* bytes) {
+  if (keep == KEEP_FEW && N > FEW_ROWS) return set_error(CPB_ERR_ARG, "objective: %d rows are not few", N);
   if (N <= 0 || d <= 0 || V <= 0 || chunk <= 0 || chunk % 256) return set_error(CPB_ERR_ARG, "objective: %d rows of %d, %d columns, chunks of %d", N, d, V, chunk);
   size_t kept, bwd;
-  rows_layout(nullptr, N, d, V, chunk, store, kept);
-  fwd_layout(nullptr, N, d, V, chunk, store, kept);
-  bwd_layout(nullptr, N, d, V, chunk, dw, want_dx, bwd);
+  rows_layout(nullptr, N, d, V, chunk, keep, kept);
+  fwd_layout(nullptr, N, d, V, chunk, keep, kept);
+  bwd_layout(nullptr, N, d, V, chunk, keep, dw, want_dx, bwd);
   bytes[0] = (int64_t)kept; bytes[1] = (int64_t)bwd;
   return CPB_OK;
 }
 
-static int objective_args(int N, int d, int V, int n_valid, int ldw, int chunk) {
+static int objective_args(int N, int d, int V, int n_valid, int ldw, int chunk, int keep) {
+  if (keep < KEEP_NONE || keep > KEEP_FEW || (keep == KEEP_FEW && N > FEW_ROWS)) return set_error(CPB_ERR_ARG, "objective: %d rows kept as %d", N, keep);
   if (N <= 0 || d <= 0 || V <= 0) return set_error(CPB_ERR_ARG, "objective: empty problem, %d rows of %d, %d columns", N, d, V);
   if ((d % 8) || (V % 8) || (ldw % 8)) return set_error(CPB_ERR_ARG, "objective: widths and row strides must be multiples of 8 (got d=%d V=%d ldw=%d)", d, V, ldw);
   if (n_valid <= 0 || n_valid > V) return set_error(CPB_ERR_ARG, "objective: n_valid=%d outside 1..%d", n_valid, V);
@@ -572,18 +608,18 @@ static int objective_args(int N, int d, int V, int n_valid, int ldw, int chunk) 
 // last two may be null), loss [1] and terms [4], see Policy.  kept: cpb_objective_plan.
 extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, int d, const void* w, int ldw, int V, int n_valid, const int64_t* targets,
                                  const float* old_logp, const float* advantages, const float* weights, const float* ref_logp, double low, double high,
-                                 double kl, float* logp, float* loss, float* terms, void* kept, int store, int chunk, int* status, cudaStream_t stream) {
-  int rc = objective_args(N, d, V, n_valid, ldw, chunk);
+                                 double kl, float* logp, float* loss, float* terms, void* kept, int keep, int chunk, int* status, cudaStream_t stream) {
+  int rc = objective_args(N, d, V, n_valid, ldw, chunk, keep);
   if (rc != CPB_OK) return rc;
   if (T <= 0 || N % T || (sb % 8) || (st % 8) || ((uintptr_t)x & 15)) return set_error(CPB_ERR_ARG, "objective: hidden states need 16-byte aligned rows");
   size_t bytes;
-  const Rows r = rows_layout((char*)kept, N, d, V, chunk, store, bytes);
-  const FwdScratch s = fwd_layout((char*)kept, N, d, V, chunk, store, bytes);
-  const int groups = (N + 31) / 32, tiles = (V + 255) / 256 * head_parts(d);
+  const Rows r = rows_layout((char*)kept, N, d, V, chunk, keep, bytes);
+  const FwdScratch s = fwd_layout((char*)kept, N, d, V, chunk, keep, bytes);
+  const int groups = (N + 31) / 32, tiles = (V + 255) / 256 * (keep ? 1 : head_parts(d));
   const bool count = N <= COUNT_ROWS;
   if (!count) CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
   auto gather = count ? rows_gather_kernel<true> : rows_gather_kernel<false>;
-  CPB_CUDA_OK(launch_pdl(gather, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, logp, r, dx_ranges(N < chunk ? N : chunk, d, V),
+  CPB_CUDA_OK(launch_pdl(gather, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, logp, r, dx_ranges(r.half ? 2 * r.half : N < chunk ? N : chunk, d, V),
                          chunk, N, n_valid, status));
   int blocks = 0;
   for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
@@ -591,9 +627,9 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, loss, terms};
   for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
-    float2* stats = store ? r.stats + (size_t)tiles * r0 : s.stats;
+    float2* stats = keep ? r.stats + (size_t)tiles * r0 : s.stats;
     const HeadParams head{r.targets + r0, stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, (float)(logits * 1.4426950408889634)};
-    if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, store ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, store ? 2 : 0, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
+    if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, keep ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, keep ? 2 : 0, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     auto kern = advantages ? rows_finish_kernel<true> : rows_finish_kernel<false>;
     CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, stats, s.target_logit, r, logp, r0, n, tiles, logits, q, done, blocks));
     done += (n + 31) / 32;
@@ -628,41 +664,42 @@ extern "C" int cpb_preference(const float* logp, const float* ref, const int64_t
 // Gradients: h is dloss / dlogp of row i at h[i / each] (h null: the policy loss's, as the forward pass has left it), most the largest size of
 // one or null, g a factor in device memory or null.  dx bf16 [N, d] or null.  dw: DW_ADD fp32 [V, d], added to; DW_BF16 bf16 [V, d].
 extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, int n_valid, const float* h, int each, const float* most, const float* g, void* dx, void* dw,
-                                 int dw_kind, const void* kept, int store, void* scratch, int chunk, int* status, cudaStream_t stream) {
-  int rc = objective_args(N, d, V, n_valid, ldw, chunk);
+                                 int dw_kind, const void* kept, int keep, void* scratch, int chunk, int* status, cudaStream_t stream) {
+  int rc = objective_args(N, d, V, n_valid, ldw, chunk, keep);
   if (rc != CPB_OK) return rc;
   if ((h != nullptr && each <= 0) || dw_kind < DW_NONE || dw_kind > DW_BF16 || (dw_kind != DW_NONE && dw == nullptr))
     return set_error(CPB_ERR_ARG, "objective: gradients of %d rows each, weights' gradient of kind %d", each, dw_kind);
   size_t bytes;
-  const Rows r = rows_layout((char*)kept, N, d, V, chunk, store, bytes);
-  const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, dw_kind, dx != nullptr, bytes);
+  const Rows r = rows_layout((char*)kept, N, d, V, chunk, keep, bytes);
+  const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, keep, dw_kind, dx != nullptr, bytes);
   const bool one = N <= chunk;
   const float l2e = (float)(logit_scale(d) * 1.4426950408889634);
-  const Ranges q = dx_ranges(one ? N : chunk, d, V);
+  const Ranges q = dx_ranges(r.half ? 2 * r.half : one ? N : chunk, d, V);
   if (h == nullptr) { h = r.h; each = 0; }
   const Even even{most, s.back};
   const float* back = most ? s.back : nullptr;
-  if (!store) CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h, each, g, even, s.scale, N));
+  if (!keep) CPB_CUDA_OK(launch_pdl(rows_scale_kernel, (N + 255) / 256, 256, 0, stream, r, h, each, g, even, s.scale, N));
   for (int r0 = 0, c = 0; r0 < N; r0 += chunk, ++c) {
-    const int n = N - r0 < chunk ? N - r0 : chunk;
-    if (store) {
-      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, n), 256, 0, stream, r, h, each, g, even, r0, n, s.dlogits, n_valid, V, l2e));
+    const int n = N - r0 < chunk ? N - r0 : chunk, m = r.half ? 2 * r.half : n;        // rows of x, of dlogits
+    const int* live = r.half ? r.live + 2 : r.live;
+    if (keep) {
+      CPB_CUDA_OK(launch_pdl(rows_dlogits_kernel, dim3((V + RD_COLS - 1) / RD_COLS, r.half ? r.half : n), 256, 0, stream, r, h, each, g, even, r0, n, s.dlogits, n_valid, V, l2e));
     } else {
       const HeadParams head{r.targets + r0, nullptr, nullptr, r.norm + r0, n_valid, 0.f, s.scale + r0, l2e};
       if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, s.dlogits, n, V, d, d, ldw, V, 1, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     }
     if (dx != nullptr) {
       const int bn = q.t64 == 370 ? 256 : q.t64 == 300 ? 192 : 128;
-      if ((rc = gemm_live_parts(s.dlogits, w, s.dx, n, d, V, ldw, bn, q.most, back, Live{r.live, r0, 0, r.ranges + c}, status, stream)) != CPB_OK) return rc;
+      if ((rc = gemm_live_parts(s.dlogits, w, s.dx, m, d, V, ldw, bn, q.most, back, Live{live, r0, 0, r.ranges + c}, status, stream)) != CPB_OK) return rc;
       const size_t total = (size_t)N * (d / 8), blocks = (total + 255) / 256, cap = (size_t)sm_count() * 8;
-      CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, r.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, n, total));
+      CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, r.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, m, r.half, total));
     }
     if (dw_kind != DW_NONE) {
       const bool direct = dw_kind == DW_BF16 && one;
       const int epi = direct ? EPI_BF16 : dw_kind == DW_BF16 && r0 == 0 ? EPI_F32 : EPI_F32_ACC;
-      GemmLive m{s.dlogits, r.x + (size_t)r0 * d, dw_kind == DW_BF16 && !one ? (void*)s.dw : dw, V, d, n, V, d, d, 1, 1, epi, back, s.partials,
-                 epi == EPI_F32 ? 1 : gemm_splits(V, d, n, epi)};
-      if ((rc = gemm_live(m, Live{r.live, r0, 1, nullptr}, status, stream)) != CPB_OK) return rc;
+      GemmLive p{s.dlogits, r.x + (size_t)r0 * d, dw_kind == DW_BF16 && !one ? (void*)s.dw : dw, V, d, m, V, d, d, 1, 1, epi, back, s.partials,
+                 epi == EPI_F32 ? 1 : gemm_splits(V, d, m, epi)};
+      if ((rc = gemm_live(p, Live{live, r0, 1, nullptr}, status, stream)) != CPB_OK) return rc;
     }
   }
   if (dw_kind == DW_BF16 && !one) {

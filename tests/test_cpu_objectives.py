@@ -189,14 +189,17 @@ def test_plans():
     for N, d, V in ((1, 8, 8), (136, 768, 50304), (8192, 2048, 128256), (131072, 64, 50304)):
         chunk = O._chunk(V)
         assert chunk % 256 == 0 and 256 <= chunk <= 65280
-        for store in (False, True):
-            kept, bwd = O._plan(N, d, V, chunk, store, 2, True)
-            assert kept >= N * (4 + 4 + 8 + 8 + 4 + 2 * d + 2 * V * store) + (V + 255) // 256 * min(N, chunk) * 8 and kept % 256 == 0
-            assert bwd >= min(N, chunk) * V * 2 + min(N, chunk) * d * 4 * 2
-        assert O._plan(N, d, V, chunk, False, 0, False)[1] < bwd
+        for keep in range(3 if N <= O.FEW_ROWS else 2):
+            rows = min(N, chunk) if keep < 2 else 2 * (-(-N // 64) * 64)
+            kept, bwd = O._plan(N, d, V, chunk, keep, 2, True)
+            assert kept >= N * (4 + 4 + 8 + 8 + 4 + 2 * V * (keep > 0)) + max(N, rows * (keep > 1)) * 2 * d + (V + 255) // 256 * min(N, chunk) * 8
+            assert kept % 256 == 0 and bwd >= rows * V * 2 + rows * d * 4 * 2
+        assert O._plan(N, d, V, chunk, 0, 0, False)[1] < bwd
+    with pytest.raises(nv.NativeError):
+        O._plan(O.FEW_ROWS + 1, 64, 64, 256, 2, 2, True)
     for bad in ((0, 8, 8, 256), (1, 0, 8, 256), (1, 8, 0, 256), (1, 8, 8, 0), (1, 8, 8, 100)):
         with pytest.raises(nv.NativeError):
-            O._plan(*bad, False, 2, True)
+            O._plan(*bad, 0, 2, True)
 
 
 def _engine(**kw):

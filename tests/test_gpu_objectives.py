@@ -43,9 +43,12 @@ class _Exact:
         self.tol = 1e-5 * (1 + float(z.abs().max()))
         lp = torch.log_softmax(z, 1)
         self.p = lp.exp()
+        few = self.on.numel() <= O.FEW_ROWS
         # From a width on, the distance of a logit to its tile's maximum is kept in f16, half a step 2^-11 of the distance, which is no more than
         # that to the row's maximum: the probability changes by a factor of e to that at most, (1 + 2 x) for x below a half.
-        self.kept = (2 * 2.0 ** -11 * (z.amax(1, keepdim=True) - z)).clamp(max=1) if x.shape[-1] > O.KEEP_ABOVE and O.KEEP_BYTES else 0.0 * z
+        self.kept = (2 * 2.0 ** -11 * (z.amax(1, keepdim=True) - z)).clamp(max=1) if (x.shape[-1] > O.KEEP_ABOVE or few) and O.KEEP_BYTES else 0.0 * z
+        # few rows: what the rounding of dlogits leaves, 2^-8 of them at most, is rounded in its turn
+        self.dz = BF16 * BF16 if few and O.KEEP_BYTES else BF16
         self.logp = torch.where(self.on, lp.gather(1, self.t.clamp(min=0)[:, None])[:, 0], 0.0)
         self.V, self.shape = w.shape[0], x.shape
 
@@ -57,7 +60,7 @@ class _Exact:
         dz.scatter_add_(1, self.t.clamp(min=0)[:, None], h[:, None])
         kept = self.kept * h.abs()[:, None] * self.p
         kept.scatter_(1, self.t.clamp(min=0)[:, None], 0.0)          # the target's probability is kept in fp32
-        off = BF16 * dz.abs() + 3 * self.tol * size[:, None] * self.p + kept * (1 + BF16)
+        off = self.dz * dz.abs() + 3 * self.tol * size[:, None] * self.p + kept * (1 + self.dz)
         off.scatter_add_(1, self.t.clamp(min=0)[:, None], 3 * self.tol * size[:, None])
         dx, dw = dz @ self.w, torch.zeros(self.V, self.x.shape[1], dtype=torch.float64, device="cuda")
         ex, ew = off @ self.w.abs(), torch.zeros_like(dw)
