@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 from .. import _native as nv
 from .gemm import EPI_BF16, EPI_F32_ACC, acc_splits
 
-CHUNK_BYTES = 2 << 30            # of bf16 dlogits, the rows that go through the gradient's products at a time
+CHUNK_BYTES = 4 << 30            # of bf16 dlogits, the rows that go through the gradient's products at a time
 KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward to the backward pass
 # Width of the hidden states above which that is faster than to compute them again (and the head's GEMM has an epilogue that does).
 KEEP_ABOVE = 512

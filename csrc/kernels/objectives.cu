@@ -85,8 +85,10 @@ __device__ __forceinline__ int ranges_of(const Ranges& q, int rows) {
 }
 
 // Gathers 32 rows per block: x[b, t] has strides sb and st.  Bound by memory, 2 d bytes in and out per row.  COUNT: every block counts the
-// rows in front of its own by itself and there is no rows_count, up to COUNT_ROWS rows: 136 rows of 768 11 us for both kernels, 7 for one.
+// rows in front of its own by itself and there is no rows_count, up to COUNT_ROWS rows; eight rows per block, one for each warp: 136 rows of
+// 768 11 us for both kernels, 8 for this one.
 constexpr int COUNT_ROWS = 4096;
+constexpr int gather_rows(bool count) { return count ? 8 : 32; }
 template <bool COUNT>
 __global__ void __launch_bounds__(256)
 rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T, int d, const int64_t* __restrict__ targets,
@@ -94,11 +96,12 @@ rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T,
                    int* status) {
   pdl_release();
   pdl_wait();
-  __shared__ int part[8], s_base, s_n, s_from[32];
+  constexpr int EACH = gather_rows(COUNT);
+  __shared__ int part[8], s_base, s_n, s_from[EACH];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = blockIdx.x;
   int before = 0;
   if (COUNT) {
-    for (int i = threadIdx.x; i < group * 32; i += 256) before += row_counts(targets, weights, i, n_valid);
+    for (int i = threadIdx.x; i < group * EACH; i += 256) before += row_counts(targets, weights, i, n_valid);
   } else {
     for (int i = threadIdx.x; i < group; i += 256) before += counts[i];
   }
@@ -109,7 +112,7 @@ rows_gather_kernel(const __nv_bfloat16* __restrict__ x, long sb, long st, int T,
   if (warp == 0) {
     int base = 0;
     for (int i = 0; i < 8; ++i) base += part[i];
-    const int row = group * 32 + lane;
+    const int row = lane < EACH ? group * EACH + lane : N;
     const bool on = row < N && row_counts(targets, weights, row, n_valid);
     const unsigned mask = __ballot_sync(0xffffffffu, on);
     const int rank = __popc(mask & ((1u << lane) - 1u));
@@ -430,47 +433,32 @@ rows_dlogits_kernel(Rows r, const float* __restrict__ h, int each, const float* 
 }
 
 // dx of the rows of one chunk: the gathered row's, the sum of its parts in their order; with the first chunk the rows that do not count, 0.
-// Eight columns per thread, bound by the parts' way through L2.
+// Four columns per thread and eight parts on their way, bound by the parts' way through L2.
 __global__ void __launch_bounds__(256)
 rows_scatter_kernel(const float* __restrict__ parts, const int* __restrict__ ranges, const int* __restrict__ place, __nv_bfloat16* __restrict__ out,
                     int N, int d, int before, int rows, int half, size_t total) {
   pdl_release();
   pdl_wait();
-  const int count = *ranges, nvec = d >> 3;
-  const size_t step = (size_t)rows * d / 4;
+  const int nvec = d >> 2, count = *ranges, all = half ? 2 * count : count;        // few rows: the rounded rows' parts, then the others'
+  const size_t step = (size_t)rows * nvec, low = (size_t)half * nvec;
   for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
     const int row = (int)(i / nvec), c = (int)(i - (size_t)row * nvec), to = place[row], at = to - before;
     if (to < 0 ? before > 0 : at < 0 || at >= rows) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (to >= 0) {
-      const float4* src = (const float4*)(parts + (size_t)at * d) + 2 * c;
-      a = src[0]; b = src[1];
-      if (half) {
-        const float4* low = src + (size_t)half * d / 4;
-        for (int s = 0; s < count; ++s) {
-          const float4 u = low[s * step], v = low[s * step + 1];
-          a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
-          b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
-        }
-      }
-      int s = 1;
-      for (; s + 3 < count; s += 4) {
-        float4 u[4], v[4];
+      const float4* src = (const float4*)parts + (size_t)at * nvec + c;
+      for (int s = 0; s < all; s += 8) {
+        float4 u[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { u[k] = src[(s + k) * step]; v[k] = src[(s + k) * step + 1]; }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          a.x += u[k].x; a.y += u[k].y; a.z += u[k].z; a.w += u[k].w;
-          b.x += v[k].x; b.y += v[k].y; b.z += v[k].z; b.w += v[k].w;
+        for (int k = 0; k < 8; ++k) {
+          u[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s + k < all) u[k] = s + k < count ? src[(s + k) * step] : src[(s + k - count) * step + low];
         }
-      }
-      for (; s < count; ++s) {
-        const float4 u = src[s * step], v = src[s * step + 1];
-        a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
-        b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { a.x += u[k].x; a.y += u[k].y; a.z += u[k].z; a.w += u[k].w; }
       }
     }
-    *(uint4*)(out + (size_t)row * d + 8 * c) = make_uint4(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w), pack_bf16(b.x, b.y), pack_bf16(b.z, b.w));
+    *(uint2*)(out + (size_t)row * d + 4 * c) = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
   }
 }
 
@@ -615,9 +603,10 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
   size_t bytes;
   const Rows r = rows_layout((char*)kept, N, d, V, chunk, keep, bytes);
   const FwdScratch s = fwd_layout((char*)kept, N, d, V, chunk, keep, bytes);
-  const int groups = (N + 31) / 32, tiles = (V + 255) / 256 * (keep ? 1 : head_parts(d));
+  const int tiles = (V + 255) / 256 * (keep ? 1 : head_parts(d));
   const bool count = N <= COUNT_ROWS;
   if (!count) CPB_CUDA_OK(launch_pdl(rows_count_kernel, (N + 255) / 256, 256, 0, stream, targets, weights, s.counts, logp, r.live, N, n_valid, status));
+  const int groups = (N + gather_rows(count) - 1) / gather_rows(count);
   auto gather = count ? rows_gather_kernel<true> : rows_gather_kernel<false>;
   CPB_CUDA_OK(launch_pdl(gather, groups, 256, 0, stream, (const __nv_bfloat16*)x, sb, st, T, d, targets, weights, s.counts, logp, r, dx_ranges(r.half ? 2 * r.half : N < chunk ? N : chunk, d, V),
                          chunk, N, n_valid, status));
@@ -691,7 +680,7 @@ extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, in
     if (dx != nullptr) {
       const int bn = q.t64 == 370 ? 256 : q.t64 == 300 ? 192 : 128;
       if ((rc = gemm_live_parts(s.dlogits, w, s.dx, m, d, V, ldw, bn, q.most, back, Live{live, r0, 0, r.ranges + c}, status, stream)) != CPB_OK) return rc;
-      const size_t total = (size_t)N * (d / 8), blocks = (total + 255) / 256, cap = (size_t)sm_count() * 8;
+      const size_t total = (size_t)N * (d / 4), blocks = (total + 255) / 256, cap = (size_t)sm_count() * 8;
       CPB_CUDA_OK(launch_pdl(rows_scatter_kernel, (unsigned)(blocks < cap ? blocks : cap), 256, 0, stream, s.dx, r.ranges + c, r.place, (__nv_bfloat16*)dx, N, d, r0, m, r.half, total));
     }
     if (dw_kind != DW_NONE) {
