@@ -9,6 +9,7 @@ back to PyTorch silently.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -79,6 +80,14 @@ def stream_ptr(device=None) -> int:
     """The calling thread's current stream on ``device`` as an address (no ``torch.cuda.Stream`` object is made)."""
     idx = None if device is None else (device if isinstance(device, torch.device) else torch.device(device)).index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """Launchers run on the current device: a context in which that is ``device``."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> int:

@@ -172,7 +172,7 @@ class TrainEngine:
         ``token_logprobs`` returns them) and one value per sequence are taken as they are."""
         if v is None:
             return None
-        v = v.to(self.device, torch.float32, non_blocking=True)
+        v = self._taken(v).to(self.device, torch.float32, non_blocking=True)
         if v.dim() == 1:
             v = v[:, None]
         B, T = shape
@@ -186,7 +186,7 @@ class TrainEngine:
     def token_logprobs(self, tokens, targets) -> torch.Tensor:
         """Log-probabilities of the local tokens' targets (fp32 ``[B, T/cp]``, 0 where the target is negative), without gradients: what the
         policy or a reference gives to the objectives below."""
-        idx, tgt, pos = self.shard_batch(tokens, targets)
+        idx, tgt, pos = self.shard_batch(self._taken(tokens), self._taken(targets))
         return objectives.token_logprobs(self.model.hidden(idx, pos), self.model.head_weight(), tgt, self.cfg.vocab_size)
 
     def _objective(self, tokens, targets, last: bool, scale: float, loss_of):
@@ -227,7 +227,8 @@ class TrainEngine:
         rank of a context-parallel group."""
         def loss_of(h, w, tgt, whole):
             pairs = tgt.shape[0] // 2
-            wt = torch.full((pairs,), 1.0 / max(1, pairs), device=self.device) if weights is None else weights.to(self.device, torch.float32, non_blocking=True)
+            wt = (torch.full((pairs,), 1.0 / max(1, pairs), device=self.device) if weights is None
+                  else self._taken(weights).to(self.device, torch.float32, non_blocking=True))
             group = None
             if self.cp.cp_size > 1:
                 group = [self.cp.cp_group] if self.cp.cp_group is not None else [g for g in (self.cp.ring_group, self.cp.ulysses_group) if g is not None]

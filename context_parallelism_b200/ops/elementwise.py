@@ -121,7 +121,8 @@ def dropout(x: torch.Tensor, drop: Dropout) -> torch.Tensor:
         return x
     if x.is_cuda:
         assert x.dtype == torch.bfloat16, f"the kernels compute in bf16 (got {x.dtype})"
-        return _DropoutFn.apply(x, drop.seed, drop.pos, drop)
+        with nv.on(x.device):
+            return _DropoutFn.apply(x, drop.seed, drop.pos, drop)
     return ref.dropout(x, drop)
 
 

@@ -12,7 +12,6 @@ are padding.  Gradients of ``w`` are added to ``w.main_grad`` when it has one.  
 CPU tensors take the plain form."""
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import NamedTuple, Optional, Tuple
@@ -97,11 +96,6 @@ def _chunk(V: int) -> int:
     return min(65280, max(256, CHUNK_BYTES // (2 * V) // 256 * 256))
 
 
-def _on(device: torch.device):
-    """The launchers ask for the current device's properties."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
 class _Head:
     """What the backward pass needs of the forward pass beside the hidden states' and weights' own gradients."""
 
@@ -127,7 +121,7 @@ def _forward(x, w, targets, n_valid, grad, policy=None):
         loss, terms = torch.empty((), dtype=torch.float32, device=x.device), torch.empty(4, dtype=torch.float32, device=x.device)
     if head.N == 0:
         return head, None, logp, loss if loss is None else loss.zero_(), terms if terms is None else terms.zero_()
-    xr = x if x.dim() <= 3 and _rows16(x) else x.contiguous() if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.contiguous().clone()
+    xr = x if x.dim() <= 3 and _rows16(x) else _dense16(x)
     if xr.dim() == 3:
         T, sb, st = xr.shape[1], xr.stride(0), xr.stride(1)
     else:
@@ -142,14 +136,20 @@ def _forward(x, w, targets, n_valid, grad, policy=None):
     return head, kept, logp, loss, terms
 
 
+def _dense16(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _weights(w):
-    return w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] and _rows16(w) else w.contiguous() if w.data_ptr() % 16 == 0 or not w.is_contiguous() else w.clone()
+    return w if w.stride(0) >= w.shape[1] and _rows16(w) else _dense16(w)
 
 
 def _backward(head, kept, w, h, each, most, g, want_dx, want_dw):
     """``dx`` and ``dw`` (None where it went to ``main_grad``) from ``dloss / dlogp``, of which ``most`` is the address of the largest size, or 0."""
     dx = torch.empty(head.shape, dtype=torch.bfloat16, device=w.device) if want_dx else None
     mg = getattr(head.w, "main_grad", None) if want_dw else None
+    assert mg is None or (mg.dtype == torch.float32 and mg.is_contiguous() and mg.numel() == w.numel() and mg.device == w.device), "main_grad is fp32 and dense"
     own = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device) if want_dw and mg is None else None
     kind = 0 if not want_dw else 1 if mg is not None else 2
     if kept is None:                                                 # no tokens
@@ -250,7 +250,7 @@ def token_logprobs(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, n_va
     """``log softmax(x w^T)[target]`` (fp32, ``targets``' shape; 0 where the target is negative), with the gradient of whatever is made of it."""
     targets, n_valid = _checked(x, w, targets, n_valid)
     if x.is_cuda:
-        with _on(x.device):
+        with nv.on(x.device):
             return _LogprobsFn.apply(x, w, targets, n_valid)
     return _plain_logprobs(x, w, targets, n_valid)
 
@@ -271,7 +271,7 @@ def linear_policy_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, 
     assert 0.0 <= low <= 1.0 and 0.0 <= high < float("inf"), f"clip={clip}"
     assert 0.0 <= kl < float("inf") and (ref is not None or kl == 0.0), f"kl_coef={kl_coef} with{'out' if ref is None else ''} reference log-probabilities"
     if x.is_cuda:
-        with _on(x.device):
+        with nv.on(x.device):
             return PolicyLoss(*_PolicyFn.apply(x, w, targets, n_valid, (old, adv, wt, ref, 1.0 - low, 1.0 + high, kl)))
     return _plain_policy(x, w, targets, n_valid, old, adv, wt, ref, 1.0 - low, 1.0 + high, kl)
 
@@ -295,7 +295,7 @@ def linear_preference_loss(x: torch.Tensor, w: torch.Tensor, targets: torch.Tens
     assert 0.0 < beta < float("inf") and 0.0 <= smoothing <= 1.0, f"beta={beta}, smoothing={smoothing}"
     if x.is_cuda:
         assert x.shape[0] <= 65535, f"{x.shape[0]} sequences in one call"
-        with _on(x.device):
+        with nv.on(x.device):
             return PreferenceLoss(*_PreferenceFn.apply(x, w, targets, n_valid, ref, weights, beta, smoothing, group))
     return _plain_preference(x, w, targets, n_valid, ref, weights, beta, smoothing, group)
 
@@ -321,7 +321,7 @@ def _plain_policy(x, w, targets, n_valid, old, adv, wt, ref, low, high, kl_coef)
     surrogate = -torch.where(cut, r.detach().clamp(low, high), torch.where(cut, 0.0, r)) * adv
     kl = torch.zeros_like(lp) if ref is None else torch.expm1(ref[on].double() - lp) - (ref[on].double() - lp)
     terms = torch.stack([(wt * v).sum() for v in (surrogate, kl, cut.double(), torch.ones_like(lp))])
-    return PolicyLoss((terms[0] + kl_coef * terms[1]).to(logp.dtype), logp.detach(), terms.detach().to(logp.dtype))
+    return PolicyLoss((terms[0] + kl_coef * terms[1] if kl_coef else terms[0]).to(logp.dtype), logp.detach(), terms.detach().to(logp.dtype))
 
 
 class _SumOver(torch.autograd.Function):
@@ -346,5 +346,6 @@ def _plain_preference(x, w, targets, n_valid, ref, weights, beta, smoothing, gro
         keep = weights != 0
         chosen, rejected, weights = chosen[keep], rejected[keep], weights[keep].double()
     z = beta * (chosen - rejected)
-    each = (1 - smoothing) * torch.nn.functional.softplus(-z) + smoothing * torch.nn.functional.softplus(z)
+    sides = ((1 - smoothing, -z), (smoothing, z))                    # what counts nothing is left out, infinite or not
+    each = sum(k * torch.nn.functional.softplus(v) for k, v in sides if k)
     return PreferenceLoss((each if weights is None else each * weights).sum().to(logp.dtype), logp.detach(), ratios.detach().to(logp.dtype))

@@ -633,13 +633,13 @@ int gemm_head_live(const void* x, const void* w, void* out, int M, int N, int K,
 }
 int gemm_live_parts(const void* A, const void* w, float* parts, int M, int N, int K, int ldw, int bn, int most, const float* factor, const Live& live,
                     int* status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) || (K % 8) || (ldw % 8) || most < 2) return set_error(CPB_ERR_ARG, "gemm_live_parts: %dx%dx%d in %d", M, N, K, most);
+  if (M <= 0 || N <= 0 || K <= 0 || (N % 8) || (K % 8) || (ldw % 8) || most < 1) return set_error(CPB_ERR_ARG, "gemm_live_parts: %dx%dx%d in %d", M, N, K, most);
   GemmParams p{};
   p.M = M; p.N = N; p.K = K; p.epi = EPI_F32;
   p.num_m_tiles = (M + 2 * GEMM_BM - 1) / (2 * GEMM_BM);
   p.num_n_blocks = (N + bn - 1) / bn;
   p.num_k_blocks = (K + GEMM_BK - 1) / GEMM_BK;
-  p.splits = most;
+  p.splits = most > 1 ? most : 2;               // more than one: results go to the parts; *live.splits is at most `most`
   p.k_per_split = (p.num_k_blocks + most - 1) / most;
   p.band = tile_band(N, K);
   p.status = status;

@@ -226,7 +226,7 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
         if (q.ref_logp) {
           const double delta = (double)q.ref_logp[from] - lp, e = expm1(delta);
           kl = e - delta;
-          h -= q.kl * e;
+          if (q.kl != 0.) h -= q.kl * e;
         }
         r.h[at] = (float)(wt * h);
         sur *= wt; kl *= wt; cut = c ? wt : 0.;
@@ -266,7 +266,7 @@ rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ t
   if (threadIdx.x != 0) return;
   for (int w = 1; w < RF_WARPS; ++w)
     for (int k = 0; k < 4; ++k) total[0][k] += total[w][k];
-  *q.loss = (float)(q.ref_logp ? total[0][0] + q.kl * total[0][1] : total[0][0]);
+  *q.loss = (float)(q.kl != 0. ? total[0][0] + q.kl * total[0][1] : total[0][0]);
   for (int k = 0; k < 4; ++k) q.terms[k] = (float)total[0][k];
 }
 
@@ -321,7 +321,8 @@ preference_kernel(const double* __restrict__ sums, int parts, int pairs, const f
       // softplus(-z) = max(-z, 0) + log1p(e^-|z|); its derivative -sigma(-z)
       const double z = beta * (c - r), e = exp(-fabs(z)), small = log1p(e), pos = 1. / (1. + e), neg = e / (1. + e);
       const double up = z > 0. ? pos : z <= 0. ? neg : z, down = z > 0. ? neg : z <= 0. ? pos : z;      // sigma(z), sigma(-z); NaN stays
-      l += wt * ((1. - smoothing) * (fmax(-z, 0.) + small) + smoothing * (fmax(z, 0.) + small));
+      // a side that counts nothing is left out, infinite or not
+      l += wt * ((smoothing < 1. ? (1. - smoothing) * (fmax(-z, 0.) + small) : 0.) + (smoothing > 0. ? smoothing * (fmax(z, 0.) + small) : 0.));
       g = wt * beta * (smoothing * up - (1. - smoothing) * down);
     }
     h[i] = (float)g; h[pairs + i] = (float)-g;
@@ -520,7 +521,7 @@ static FwdScratch fwd_layout(char* base, long N, int d, long V, int chunk, int k
 }
 // Where dw goes: nowhere, added to an fp32 buffer, or as bf16 (through an fp32 buffer where there are several chunks of rows).
 enum : int { DW_NONE = 0, DW_ADD = 1, DW_BF16 = 2 };
-// Tiles of the product dz w: the width that covers d in the least time.  At most 512 MB of partial results.
+// Tiles of the product dz w: the width that covers d in the least time.  At most 512 MB of partial results, or one of them.
 static Ranges dx_ranges(int rows, int d, int V) {
   Ranges q{};
   long best = 0;
@@ -530,7 +531,7 @@ static Ranges dx_ranges(int rows, int d, int V) {
   }
   q.k_blocks = (V + GEMM_BK - 1) / GEMM_BK;
   const long most = (128L << 20) / ((long)rows * d);
-  q.most = (int)(most < 2 ? 2 : most > 32 ? 32 : most);
+  q.most = (int)(most < 1 ? 1 : most > 32 ? 32 : most);
   q.pairs = sm_count() > 1 ? sm_count() / 2 : 1;
   q.d = d;
   return q;

@@ -133,7 +133,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(nv, "call", lambda name, *a: made.append(name))
     monkeypatch.setattr(nv, "status_for", lambda dev: _Status)
     monkeypatch.setattr(nv, "stream_ptr", lambda dev=None: 0)
-    monkeypatch.setattr(O, "_on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(nv, "on", lambda dev: contextlib.nullcontext())
     return made
 
 
@@ -258,3 +258,27 @@ def test_engine_refuses():
             eng.preference_forward_backward(x, y, bad)
     with pytest.raises(AssertionError):
         eng.preference_forward_backward(x[:3], y[:3], z[:3])
+
+
+def test_what_counts_nothing_may_be_infinite():
+    """A reference that gives a token no chance: without a KL coefficient it has no part in the loss, and a pair that it decides is decided."""
+    x, w, t, g = _case(dtype=torch.float32)
+    z, ref = torch.zeros(4, 5), torch.full((4, 5), -3.0)
+    ref[0, 4] = -float("inf")
+    a, b = O.linear_policy_loss(x, w, t, z - 3, z + 1, ref_logp=ref, n_valid=21), O.linear_policy_loss(x, w, t, z - 3, z + 1, n_valid=21)
+    assert torch.equal(a.loss, b.loss) and float(a.terms[1]) == float("inf")
+    for p, q in zip(torch.autograd.grad(a.loss, [x, w]), torch.autograd.grad(b.loss, [x, w])):
+        assert torch.equal(p, q)
+    out = O.linear_preference_loss(x, w, t, ref, n_valid=21)
+    rest = torch.nn.functional.softplus(-0.1 * (out.ratios[1] - out.ratios[3]))
+    assert float(out.loss) == pytest.approx(float(rest), rel=1e-6)
+
+
+def test_main_grad_has_to_be_dense(calls):
+    x, w = _t(2, 6, 64), _t(16, 64).requires_grad_()
+    for bad in (torch.zeros(16, 64, dtype=torch.bfloat16), torch.zeros(64, 16).T, torch.zeros(16, 32)):
+        head = O._Head(x, w, torch.zeros(2, 6, dtype=torch.int64), 16, True)
+        head.w.main_grad = bad
+        with pytest.raises(AssertionError):
+            O._backward(head, torch.zeros(1), w, None, 0, 0, None, False, True)
+    assert not calls

@@ -78,7 +78,7 @@ def _within(got, want, bound, name):
 
 # one row, less and more than a warp's, a CTA's and a pair's rows; columns in one tile, one more than a tile's, a last tile of padding only;
 # both sides of the width from which logits are stored
-SHAPES = [(1, 1, 64, 8, 8, "all"), (1, 31, 64, 64, 57, "all"), (3, 11, 72, 264, 257, "response"), (2, 65, 128, 512, 250, "scattered"),
+SHAPES = [(1, 1, 64, 8, 8, "all"), (1, 5, 8, 16, 16, "all"), (1, 300, 16, 24, 20, "scattered"), (1, 31, 64, 64, 57, "all"), (3, 11, 72, 264, 257, "response"), (2, 65, 128, 512, 250, "scattered"),
           (4, 96, 384, 1024, 1000, "response"), (2, 150, 1024, 8192, 8192, "scattered"), (2, 150, 1032, 4096, 4090, "response"),
           (1, 700, 1032, 512, 512, "scattered"), (8, 200, 384, 50304, 50257, "response"), (1, 520, 2048, 1000, 990, "all"),
           (2, 40, 64, 512, 500, "none"), *[(1, 600, 64, 264, 260, str(n)) for n in (1, 63, 64, 65, 255, 256, 257, 320, 512)],
@@ -171,8 +171,6 @@ def test_preference(B, T, d, V, n_valid, spans, smoothing, beta, chunks):
     wt = torch.rand(B // 2, device="cuda", generator=g) + 0.5
     x.requires_grad_(), w.requires_grad_()
     out = O.linear_preference_loss(x, w, t, ref, wt, beta, smoothing, n_valid)
-    up = torch.tensor(0.6, device="cuda")
-    dx, dw = torch.autograd.grad(out.loss, [x, w], up)
     diff = torch.where(e.on, e.logp - ref.reshape(-1).double(), 0.0).view(B, T)
     R, off = diff.sum(1), e.tol * e.on.view(B, T).sum(1)
     z, far = beta * (R[: B // 2] - R[B // 2:]), beta * (off[: B // 2] + off[B // 2:])
@@ -185,9 +183,12 @@ def test_preference(B, T, d, V, n_valid, spans, smoothing, beta, chunks):
     h = torch.cat([dh, -dh])[:, None].expand(B, T).reshape(-1)
     # the derivative of h with respect to z is at most weight x beta / 4
     size = h.abs() + torch.cat([wt, wt]).double()[:, None].expand(B, T).reshape(-1) * beta / 4 * torch.cat([far, far])[:, None].expand(B, T).reshape(-1) / (3 * e.tol)
-    (wx, bx), (ww, bw) = e.gradients(0.6 * h, 0.6 * size)
-    _within(dx, wx, bx, "dx")
-    _within(dw, ww, bw, "dw")
+    # the gradient is taken at a power of two, which has to go out of it again whatever comes in
+    for up in (0.6, -3.0, 2.0 ** 40, 1e-20, 0.0):
+        dx, dw = torch.autograd.grad(out.loss, [x, w], torch.tensor(up, device="cuda"), retain_graph=True)
+        (wx, bx), (ww, bw) = e.gradients(up * h, abs(up) * size)
+        _within(dx, wx, bx, f"dx at {up}")
+        _within(dw, ww, bw, f"dw at {up}")
 
 
 def _calls(x, w, t, old, adv, ref, n_valid):
@@ -393,3 +394,18 @@ def test_two_captured_graphs(kind):
             o = _calls(*s, 500)[kind]()
             for a, b in zip(got, [*o, *torch.autograd.grad(o[0], s[:2])]):
                 assert torch.equal(a, b)
+
+
+def test_what_counts_nothing_may_be_infinite():
+    x, w, t, old, adv, ref = _setup(64)
+    ref = ref.clone()
+    ref[0, 100] = -float("inf")
+    assert int(t[0, 100]) >= 0
+    a, b = (O.linear_policy_loss(x, w, t, old, adv, ref_logp=r, n_valid=500) for r in (ref, None))
+    assert torch.equal(a.loss, b.loss) and float(a.terms[1]) == float("inf")
+    for p, q in zip(torch.autograd.grad(a.loss, [x, w]), torch.autograd.grad(b.loss, [x, w])):
+        assert torch.equal(p, q)
+    out = O.linear_preference_loss(x, w, t, ref, n_valid=500)
+    rest = torch.nn.functional.softplus(-0.1 * (out.ratios[1] - out.ratios[3]).double())
+    assert float(out.loss) == pytest.approx(float(rest), rel=1e-5)
+    assert all(bool(v.isfinite().all()) for v in torch.autograd.grad(out.loss, [x, w]))

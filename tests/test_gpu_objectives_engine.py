@@ -67,3 +67,30 @@ def test_tokens_that_do_not_count_change_nothing():
     a.policy_forward_backward(x2, y, bad, adv)
     # embedding, norm and dQ sums in arrival order
     assert_close(a.flat.grad, one, cos=0.999999, rel=1e-3)
+
+
+def test_page_locked_buffers_may_be_written_again():
+    """What a call reads of page-locked buffers it has taken over when it returns."""
+    a, b = _engine("cuda", "llama", dropout=0.0), _engine("cuda", "llama", dropout=0.0)
+    g = torch.Generator().manual_seed(5)
+    t = torch.randint(0, 1000, (4, 201), generator=g)
+    x, y = t[:, :-1].contiguous().pin_memory(), t[:, 1:].contiguous().pin_memory()
+    vals = [(torch.randn(4, 200, generator=g) - s).pin_memory() for s in (7, 0, 7)] + [(torch.rand(4, 200, generator=g) / 800).pin_memory()]
+    pair = torch.rand(2, generator=g).pin_memory()
+    keep = [v.clone() for v in (x, y, *vals, pair)]
+    big = torch.randn(8192, 8192, device="cuda")
+    outs = []
+    for e, (x, y, old, adv, ref, wt, pw), spoil in ((a, keep, False), (b, (x, y, *vals, pair), True)):
+        for _ in range(20):
+            big = big @ big * 1e-4                                   # the device is behind
+        p = e.policy_forward_backward(x, y, old, adv, wt, ref, kl_coef=0.1, accum=2, last=False)
+        q = e.preference_forward_backward(x, y, ref, pw, accum=2)
+        lp = e.token_logprobs(x, y)
+        if spoil:
+            x.fill_(1), y.fill_(-100)
+            for v in (old, adv, ref, wt, pw):
+                v.fill_(float("nan"))
+        outs.append((p.loss, p.terms, q.loss, q.ratios, lp))
+    for u, v in zip(*outs):
+        assert torch.allclose(u, v, rtol=1e-4, atol=1e-5)
+    assert_close(a.flat.grad, b.flat.grad, cos=0.99999, rel=1e-2)
