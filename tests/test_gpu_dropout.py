@@ -138,6 +138,12 @@ def test_refused():
         E.dropout(torch.zeros(1, 4, 64, device="cuda"), drop)
     with pytest.raises(AssertionError):
         E.dropout(torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16), drop._replace(seed=drop.seed.cpu()))
+    x, w = torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16), torch.ones(68, device="cuda")
+    for bad in (w[:64].bfloat16(), w[:56], w[1:65], w[:64].cpu(), torch.ones(64, 2, device="cuda")[:, 0]):
+        with pytest.raises(AssertionError):
+            E.rmsnorm(x, bad, 1e-5, x, drop)
+        with pytest.raises(AssertionError):
+            E.layernorm(x, w[:64], bad, 1e-5, x, drop)
     with pytest.raises(NativeError):
         E.dropout(torch.zeros(1, 4, 60, device="cuda", dtype=torch.bfloat16), drop)
 
