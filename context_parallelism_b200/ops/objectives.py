@@ -68,6 +68,8 @@ def _per_token(name, t, like, optional=False):
         return None
     assert isinstance(t, torch.Tensor) and t.is_floating_point() and t.device == like.device, f"{name} must be floating-point values on {like.device}"
     assert not t.requires_grad, f"{name} is a constant of the objective and has no gradient: detach it"
+    if t.shape == like.shape:
+        return t.float().contiguous()
     assert t.dim() == like.dim(), f"{name} of {tuple(t.shape)} for tokens of {tuple(like.shape)}"
     return t.float().expand(like.shape).contiguous()
 
@@ -112,22 +114,22 @@ def _rows16(t):
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
 
 
-def _forward(x, w, targets, n_valid, grad, policy=None):
-    """Log-probabilities, what is kept for the backward pass, and for a policy loss the loss and its terms."""
+def _forward(x, w, targets, n_valid, grad, policy=None, more=0):
+    """Log-probabilities, what is kept for the backward pass (and ``more`` bytes behind it), and for a policy loss the loss and its terms."""
     head = _Head(x, w, targets, n_valid, grad)
     logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
     loss = terms = None
     if policy is not None:
         loss, terms = torch.empty((), dtype=torch.float32, device=x.device), torch.empty(4, dtype=torch.float32, device=x.device)
     if head.N == 0:
-        return head, None, logp, loss if loss is None else loss.zero_(), terms if terms is None else terms.zero_()
+        return head, torch.empty(more, dtype=torch.uint8, device=x.device), logp, loss if loss is None else loss.zero_(), terms if terms is None else terms.zero_()
     xr = x if x.dim() <= 3 and _rows16(x) else _dense16(x)
     if xr.dim() == 3:
         T, sb, st = xr.shape[1], xr.stride(0), xr.stride(1)
     else:
         T, sb, st = head.N, 0, xr.stride(-2)
     wr = _weights(w)
-    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, 0, False)[0], dtype=torch.uint8, device=x.device)
+    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, 0, False)[0] + more, dtype=torch.uint8, device=x.device)
     old, adv, weights, ref, low, high, kl = policy or (None, None, None, None, 0.0, 0.0, 0.0)
     chunks = -(-head.N // head.chunk)
     nv.LAUNCHES[0] += (head.N > COUNT_ROWS) + 2 * chunks
@@ -146,20 +148,21 @@ def _weights(w):
 
 
 def _backward(head, kept, w, h, each, most, g, want_dx, want_dw):
-    """``dx`` and ``dw`` (None where it went to ``main_grad``) from ``dloss / dlogp``, of which ``most`` is the address of the largest size, or 0."""
+    """``dx`` and ``dw`` (None where it went to ``main_grad``) from ``dloss / dlogp``, whose address is ``h``, and of which ``most`` is that of the largest
+    size, or 0."""
     dx = torch.empty(head.shape, dtype=torch.bfloat16, device=w.device) if want_dx else None
     mg = getattr(head.w, "main_grad", None) if want_dw else None
     assert mg is None or (mg.dtype == torch.float32 and mg.is_contiguous() and mg.numel() == w.numel() and mg.device == w.device), "main_grad is fp32 and dense"
     own = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device) if want_dw and mg is None else None
     kind = 0 if not want_dw else 1 if mg is not None else 2
-    if kept is None:                                                 # no tokens
+    if head.N == 0:
         if own is not None:
             own.zero_()
     elif want_dx or want_dw:
         wr = _weights(w)
         scratch = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, kind, want_dx)[1], dtype=torch.uint8, device=w.device)
         nv.LAUNCHES[0] += _backward_launches(head.N, head.d, head.V, head.chunk, head.keep, kind, want_dx) - 1
-        nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, nv.ptr(h), each, most, nv.ptr(g), nv.ptr(dx),
+        nv.call("objective_bwd", head.N, head.d, wr.data_ptr(), wr.stride(0), head.V, head.n_valid, h, each, most, nv.ptr(g), nv.ptr(dx),
                 (mg if mg is not None else own).data_ptr() if want_dw else 0, kind, kept.data_ptr(), head.keep, scratch.data_ptr(), head.chunk,
                 nv.status_for(w.device).ptr(), nv.stream_ptr(w.device))
     if mg is not None:
@@ -187,7 +190,8 @@ class _LogprobsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         w, kept = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, g.float().contiguous(), 1, 0, None, *ctx.needs_input_grad[:2])
+        g = g.float().contiguous()
+        dx, dw = _backward(ctx.head, kept, w, g.data_ptr(), 1, 0, None, *ctx.needs_input_grad[:2])
         return dx, dw, None, None
 
 
@@ -206,31 +210,36 @@ class _PolicyFn(torch.autograd.Function):
         if g is None:
             return None, None, None, None, None
         w, kept = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, None, 0, 0, g.float().contiguous(), *ctx.needs_input_grad[:2])
+        dx, dw = _backward(ctx.head, kept, w, 0, 0, 0, g.float().contiguous(), *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None
 
 
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, targets, n_valid, ref, weights, beta, smoothing, group):
-        ctx.head, kept, logp, *_ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad))
         seqs, T = targets.shape
         parts = max(1, -(-T // PART))
-        sums = torch.empty((seqs, parts), dtype=torch.float64, device=x.device)
+        more = 8 * seqs * parts + 4 * (seqs + 1)                     # the sums, and dloss / dlogp of every sequence with the largest
+        ctx.head, kept, logp, *_ = _forward(x, w, targets, n_valid, any(ctx.needs_input_grad), None, more)
         loss = torch.empty((), dtype=torch.float32, device=x.device)
-        ratios, h = torch.empty(seqs, dtype=torch.float32, device=x.device), torch.empty(seqs + 1, dtype=torch.float32, device=x.device)
+        ratios = torch.empty(seqs, dtype=torch.float32, device=x.device)
         stream = nv.stream_ptr(x.device)
+        sums = kept.data_ptr() + kept.numel() - more
+        ctx.h = 8 * seqs * parts - more
         mine = (logp.data_ptr(), ref.data_ptr(), targets.data_ptr())
-        if T == 0:
-            sums.zero_()
-        elif group is not None:
-            nv.call("sequence_sums", *mine, sums.data_ptr(), seqs, T, parts, n_valid, stream)
+        if T == 0 or group is not None:
+            t = kept[kept.numel() - more: kept.numel() + ctx.h].view(torch.float64)
+            if T == 0:
+                t.zero_()
+            else:
+                nv.call("sequence_sums", *mine, sums, seqs, T, parts, n_valid, stream)
+            _sum_over(t, group)
+            mine = (0, 0, 0)
         else:
             nv.LAUNCHES[0] += 1
-        _sum_over(sums, group)
-        nv.call("preference", *(mine if T and group is None else (0, 0, 0)), T, n_valid, sums.data_ptr(), parts, seqs // 2, nv.ptr(weights), beta, smoothing,
-                loss.data_ptr(), ratios.data_ptr(), h.data_ptr(), stream)
-        ctx.save_for_backward(w, kept, h)
+        nv.call("preference", *mine, T, n_valid, sums, parts, seqs // 2, nv.ptr(weights), beta, smoothing, loss.data_ptr(), ratios.data_ptr(),
+                sums + 8 * seqs * parts, stream)
+        ctx.save_for_backward(w, kept)
         ctx.mark_non_differentiable(logp, ratios)
         ctx.set_materialize_grads(False)
         return loss, logp, ratios
@@ -240,8 +249,9 @@ class _PreferenceFn(torch.autograd.Function):
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 9
-        w, kept, h = ctx.saved_tensors
-        dx, dw = _backward(ctx.head, kept, w, h, max(1, ctx.head.shape[1]), h[-1:].data_ptr(), g.float().contiguous(), *ctx.needs_input_grad[:2])
+        w, kept = ctx.saved_tensors
+        end = kept.data_ptr() + kept.numel()
+        dx, dw = _backward(ctx.head, kept, w, end + ctx.h, max(1, ctx.head.shape[1]), end - 4, g.float().contiguous(), *ctx.needs_input_grad[:2])
         return dx, dw, None, None, None, None, None, None, None
 
 

@@ -280,5 +280,5 @@ def test_main_grad_has_to_be_dense(calls):
         head = O._Head(x, w, torch.zeros(2, 6, dtype=torch.int64), 16, True)
         head.w.main_grad = bad
         with pytest.raises(AssertionError):
-            O._backward(head, torch.zeros(1), w, None, 0, 0, None, False, True)
+            O._backward(head, torch.zeros(1), w, 0, 0, 0, None, False, True)
     assert not calls
