@@ -171,48 +171,78 @@ struct Policy {
   float *loss, *terms;                                             // [1], and [4] sums of weight x (surrogate, KL, clipped, 1)
 };
 
+// The tensor core cuts off what an accumulator has no bits for after every 16 of K, so a logit comes out too small in size: half a last place a
+// step, for a sum that grows evenly K 2^-30 of it.  Measured at logits above 8 (spread 4, 50304 and 128256 columns), relative: K 384
+// -3.4e-7, 768 -7.0e-7, 2048 -1.97e-6, 4096 -4.05e-6; this factor takes it back.  A sum that has its size early is off by
+// up to twice that, one that gets it late by next to nothing, so it is nowhere further off with the factor than without.
+// `l2e` is it times log2 e, rounded to fp32, and `all` what that comes to: a target's logit has to take the same as the exponentials, or
+// log-probabilities are up to 2e-7 off on average.
+struct LogitScale { float l2e; double all; };
+static LogitScale logit_scale(int d) {
+  const float l2e = (float)((1. + (double)d / 1073741824.) * 1.4426950408889634);
+  return LogitScale{l2e, (double)l2e * 0.6931471805599453};
+}
+
 // Between the two passes of the head's GEMM: logp and (max, 1 / sum) of 32 gathered rows per block, and for a policy loss its terms and h.
 // A warp takes every sixteenth part of the columns (the lanes' pairs are adjacent in memory), warp 0 adds the warps', always in the same order.
+// A target's logit is the tensor core's, like those in the sum: computed exactly, logp deviates a third as much from token to token (K 4096
+// 3e-6 for 1e-5), but what the factor above does not meet then stays in every one of them (2.4e-6 there), and sums over answers are worse.
+// ex2.approx is 4.8e-8 too low on average where it is not exact, as it is for the maximum itself: the sum gets that back (logp 1e-7 too high on
+// average without, 1e-8 to 5e-8 with it).
 constexpr int RF_WARPS = 16;
+constexpr double EX2_LOW = 4.8e-8;
 template <bool POLICY>
 __global__ void __launch_bounds__(RF_WARPS * 32)
 rows_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logit, Rows r, float* __restrict__ logp, int before, int rows,
-                   int tiles, double logits, Policy q, int blocks_before, int blocks) {
+                   int tiles, LogitScale scale, Policy q, int blocks_before, int blocks) {
   pdl_release();
   pdl_wait();
-  __shared__ float2 part[RF_WARPS][32];
+  __shared__ double2 part[RF_WARPS][32];
   __shared__ int s_last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + lane;                          // in this launch
   const int at = before + row;                                     // gathered
   const bool on = row < rows && at < r.live[0];
-  float m = -INFINITY, s = 0.f;
-  const float l2e = (float)(logits * 1.4426950408889634);
+  float m = -INFINITY;
+  double s = 0.;
   // a part without a finite maximum contributes its sum as it is: zero, or NaN
-  const auto add = [&](float2 v) {
-    const float mn = fmaxf(m, v.x);
-    s = (m == -INFINITY ? s : s * ex2f((m - mn) * l2e)) + (v.x == -INFINITY ? v.y : v.y * ex2f((v.x - mn) * l2e));
-    m = mn;
-  };
+  const auto below = [&](float v, float top) { return v == top || v == -INFINITY ? 1. : (1. + EX2_LOW) * (double)ex2f((v - top) * scale.l2e); };
+  const auto given = [&](float2 v, float top) { return v.x == -INFINITY ? (double)v.y : ((double)v.y + EX2_LOW * ((double)v.y - 1.)) * below(v.x, top); };
   if (on) {
     int t = warp;
     for (; t + 7 * RF_WARPS < tiles; t += 8 * RF_WARPS) {
       float2 v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = stats[(size_t)(t + k * RF_WARPS) * rows + row];
+      float top = m;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) add(v[k]);
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, v[k].x);
+      s *= below(m, top);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += given(v[k], top);
+      m = top;
     }
-    for (; t < tiles; t += RF_WARPS) add(stats[(size_t)t * rows + row]);
+    for (; t < tiles; t += RF_WARPS) {
+      const float2 v = stats[(size_t)t * rows + row];
+      const float top = fmaxf(m, v.x);
+      s = s * below(m, top) + given(v, top);
+      m = top;
+    }
   }
-  part[warp][lane] = make_float2(m, s);
+  part[warp][lane] = make_double2((double)m, s);
   __syncthreads();
   if (warp == 0) {
-    for (int k = 1; k < RF_WARPS; ++k) add(part[k][lane]);
+    float top = m;
+#pragma unroll
+    for (int k = 1; k < RF_WARPS; ++k) top = fmaxf(top, (float)part[k][lane].x);
+    s *= below(m, top);
+#pragma unroll
+    for (int k = 1; k < RF_WARPS; ++k) s += part[k][lane].y * below((float)part[k][lane].x, top);
+    m = top;
     double sur = 0., kl = 0., cut = 0., wt = 0.;
     if (on) {
-      const double lp = logits * ((double)target_logit[row] - (double)m) - log((double)s);
-      r.norm[at] = make_float2(m, 1.f / s);
+      const double lp = scale.all * ((double)target_logit[row] - (double)m) - log(s);
+      r.norm[at] = make_float2(m, (float)(1. / s));
       r.target_p[at] = (float)exp(lp);
       const int from = r.from[at];
       logp[from] = (float)lp;
@@ -474,13 +504,6 @@ weight_cast_kernel(const float4* __restrict__ in, uint4* __restrict__ out, size_
   }
 }
 
-// The tensor core cuts off what an accumulator has no bits for after every 16 of K, so a logit comes out too small in size: half a last place a
-// step, for a sum that grows evenly K 2^-30 of it.  Measured at logits above 8 (spread 4, 50304 and 128256 columns), relative: K 384
-// -3.4e-7, 768 -7.0e-7, 2048 -1.97e-6, 4096 -4.05e-6; this factor takes it back.  A sum that has its size early is off by
-// up to twice that, one that gets it late by next to nothing, so it is nowhere further off with the factor than without.  A single logp hardly
-// shows it, target and normaliser being off alike; sums over an answer do.
-static double logit_scale(int d) { return 1. + (double)d / 1073741824.; }
-
 // ------------------------------------------------------------------ layout of the buffers
 static size_t take(size_t& at, size_t bytes) {
   const size_t here = at;
@@ -613,15 +636,15 @@ extern "C" int cpb_objective_fwd(const void* x, long sb, long st, int N, int T, 
                          chunk, N, n_valid, status));
   int blocks = 0;
   for (int r0 = 0; r0 < N; r0 += chunk) blocks += ((N - r0 < chunk ? N - r0 : chunk) + 31) / 32;
-  const double logits = logit_scale(d);
+  const LogitScale scale = logit_scale(d);
   const Policy q{old_logp, advantages, weights, ref_logp, low, high, kl, s.part, loss, terms};
   for (int r0 = 0, done = 0; r0 < N; r0 += chunk) {
     const int n = N - r0 < chunk ? N - r0 : chunk;
     float2* stats = keep ? r.stats + (size_t)tiles * r0 : s.stats;
-    const HeadParams head{r.targets + r0, stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, (float)(logits * 1.4426950408889634)};
+    const HeadParams head{r.targets + r0, stats, s.target_logit, nullptr, n_valid, 0.f, nullptr, scale.l2e};
     if ((rc = gemm_head_live(r.x + (size_t)r0 * d, w, keep ? r.logits + (size_t)r0 * V : nullptr, n, V, d, d, ldw, V, keep ? 2 : 0, head, Live{r.live, r0, 0, nullptr}, status, stream)) != CPB_OK) return rc;
     auto kern = advantages ? rows_finish_kernel<true> : rows_finish_kernel<false>;
-    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, stats, s.target_logit, r, logp, r0, n, tiles, logits, q, done, blocks));
+    CPB_CUDA_OK(launch_pdl(kern, (n + 31) / 32, RF_WARPS * 32, 0, stream, stats, s.target_logit, r, logp, r0, n, tiles, scale, q, done, blocks));
     done += (n + 31) / 32;
   }
   return check_launch("objective_fwd");
@@ -663,7 +686,7 @@ extern "C" int cpb_objective_bwd(int N, int d, const void* w, int ldw, int V, in
   const Rows r = rows_layout((char*)kept, N, d, V, chunk, keep, bytes);
   const BwdScratch s = bwd_layout((char*)scratch, N, d, V, chunk, keep, dw_kind, dx != nullptr, bytes);
   const bool one = N <= chunk;
-  const float l2e = (float)(logit_scale(d) * 1.4426950408889634);
+  const float l2e = logit_scale(d).l2e;
   const Ranges q = dx_ranges(r.half ? 2 * r.half : one ? N : chunk, d, V);
   if (h == nullptr) { h = r.h; each = 0; }
   const Even even{most, s.back};
