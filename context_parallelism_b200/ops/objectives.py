@@ -23,11 +23,18 @@ from torch.autograd.function import once_differentiable
 from .. import _native as nv
 from .gemm import EPI_BF16, EPI_F32_ACC, acc_splits
 
-CHUNK_BYTES = 4 << 30            # of bf16 dlogits, the rows that go through the gradient's products at a time
-KEEP_BYTES = 16 << 30            # of logits in 16 bits, kept from the forward to the backward pass
-# Width of the hidden states above which that is faster than to compute them again (and the head's GEMM has an epilogue that does).
+# Of bf16 dlogits, the rows that go through the gradient's products at a time: each further chunk adds its dw to an fp32 buffer, 4 bytes read and
+# written per weight (two chunks of 8192 rows, 128256 columns of 2048: 14.3 ms, one of 16384 13.9).
+CHUNK_BYTES = 4 << 30
+# Of logits in 16 bits, kept from the forward to the backward pass, a tenth of the GPU's memory; beyond, they are computed again.
+KEEP_BYTES = 16 << 30
+# Width of the hidden states above which that is faster than to compute them again.  token_logprobs and its gradient, us, kept and computed
+# again: 4608 x 50304, width 384 757 and 728 (without a pause), 512 871 and 876, 520 914 and 952, 640 918 and 967, 768 932 and 1029, 1024 1148 and
+# 1278; 4608 x 128256, 2048 5513 and 6843.
 KEEP_ABOVE = 512
-FEW_ROWS = 256                   # up to which dlogits are the sum of two bf16 numbers
+# Rows up to which dlogits are the sum of two bf16 numbers, and logits always kept.  136 rows, width 768, 50304 columns: 14 us more of the GPU's 110,
+# which a call of this size does not notice; beyond, the products would take up to twice as long.
+FEW_ROWS = 256
 PART = 4096                      # tokens of a sequence that one block adds up
 COUNT_ROWS = 4096                # up to which rows are counted and gathered in one launch
 

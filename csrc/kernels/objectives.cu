@@ -6,7 +6,7 @@
 // (rows_count, rows_gather), and the GEMMs behind read from device memory how many there are (Live in gemm_common.cuh): masked tokens cost
 // nothing, whatever they hold, and the host does not wait for the number.  Then as for the cross entropy (xent.cu): the head's GEMM leaves
 // (max, sum of exponentials) per row and part of the columns, rows_finish makes logp and h of them, and for the gradient a second GEMM
-// computes the logits again or, from a width of 520 on, rows_dlogits takes what the first has kept of them in 16 bits.  Everything per token is
+// computes the logits again or, above a width of 512, rows_dlogits takes what the first has kept of them in 16 bits.  Everything per token is
 // computed in 64 bits: e^d - d - 1 of two nearly equal log-probabilities and the sums over long answers need it, and there are few tokens.
 // Every sum has a fixed order: a call repeats bit for bit.
 #include <cuda_fp16.h>

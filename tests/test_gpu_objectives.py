@@ -409,3 +409,64 @@ def test_what_counts_nothing_may_be_infinite():
     rest = torch.nn.functional.softplus(-0.1 * (out.ratios[1] - out.ratios[3]).double())
     assert float(out.loss) == pytest.approx(float(rest), rel=1e-5)
     assert all(bool(v.isfinite().all()) for v in torch.autograd.grad(out.loss, [x, w]))
+
+
+@pytest.mark.parametrize("kind", ["policy", "preference", "logprobs"])
+def test_threads_modes_and_recomputation(kind):
+    """Calls of two threads on streams of their own, without autograd, and recomputed by a checkpoint."""
+    import threading
+
+    from torch.utils.checkpoint import checkpoint
+    sets = [_setup(1032), _setup(64, T=200)]
+    want = []
+    for s in sets:
+        o = _calls(*s, 500)[kind]()
+        want.append([*(v.detach() for v in o), *torch.autograd.grad(o[0], s[:2])])
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    o = _calls(*sets[i], 500)[kind]()
+                    got[i] = [*(v.detach() for v in o), *torch.autograd.grad(o[0], sets[i][:2])]
+            st.synchronize()
+        except Exception as e:                                       # shown by the assertion below
+            errors.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for s, w in zip(sets, want):
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                assert all(torch.equal(p, q) for p, q in zip(_calls(*s, 500)[kind](), w))
+        x, rest = s[0], s[1:]
+        loss = checkpoint(lambda x: _calls(x, *rest, 500)[kind]()[0], x, use_reentrant=False)
+        for p, q in zip(torch.autograd.grad(loss, s[:2]), w[-2:]):
+            assert torch.equal(p, q)
+
+
+def test_more_than_two_to_the_31_logits():
+    """Offsets of kept logits and dlogits pass 32 bits; the same rows in two calls give the same."""
+    B, T, d, V = 2, 8600, 520, 128256
+    x, w, t, g = _case(B, T, d, V, V, "all")
+    assert B * T * V > 1 << 31
+    x.requires_grad_(), w.requires_grad_()
+    u = torch.randn(B, T, device="cuda", generator=g)
+    logp = O.token_logprobs(x, w, t)
+    dx, dw = torch.autograd.grad(logp, [x, w], u)
+    parts = [O.token_logprobs(x[b], w, t[b]) for b in range(2)]
+    grads = [torch.autograd.grad(p, [x, w], u[b]) for b, p in enumerate(parts)]
+    assert torch.equal(logp, torch.stack(parts))
+    # dx: the same dlogits, their products added in other ranges of K and rounded once more to bf16; dw: halves that were rounded each
+    whole = sum(g[0] for g in grads).double()
+    assert float((dx.double() - whole).norm() / whole.norm()) < BF16
+    whole = sum(g[1].double() for g in grads)
+    assert float((dw.double() - whole).norm() / whole.norm()) < 2 * BF16
