@@ -26,7 +26,8 @@ from .gemm import EPI_BF16, EPI_F32_ACC, acc_splits
 # Of bf16 dlogits, the rows that go through the gradient's products at a time: each further chunk adds its dw to an fp32 buffer, 4 bytes read and
 # written per weight (two chunks of 8192 rows, 128256 columns of 2048: 14.3 ms, one of 16384 13.9).
 CHUNK_BYTES = 4 << 30
-# Of logits in 16 bits, kept from the forward to the backward pass, a tenth of the GPU's memory; beyond, they are computed again.
+# Of logits in 16 bits, kept from the forward to the backward pass, a tenth of the GPU's memory; beyond, and where there is no room, they are
+# computed again.
 KEEP_BYTES = 16 << 30
 # Width of the hidden states above which that is faster than to compute them again.  token_logprobs and its gradient, us, kept and computed
 # again: 4608 x 50304, width 384 757 and 728 (without a pause), 512 871 and 876, 520 914 and 952, 640 918 and 967, 768 932 and 1029, 1024 1148 and
@@ -136,7 +137,13 @@ def _forward(x, w, targets, n_valid, grad, policy=None, more=0):
     else:
         T, sb, st = head.N, 0, xr.stride(-2)
     wr = _weights(w)
-    kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, 0, False)[0] + more, dtype=torch.uint8, device=x.device)
+    try:
+        kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, head.keep, 0, False)[0] + more, dtype=torch.uint8, device=x.device)
+    except torch.OutOfMemoryError:
+        if not head.keep:
+            raise
+        head.keep = 0                                                # no room for logits: they are computed again
+        kept = torch.empty(_plan(head.N, head.d, head.V, head.chunk, 0, 0, False)[0] + more, dtype=torch.uint8, device=x.device)
     old, adv, weights, ref, low, high, kl = policy or (None, None, None, None, 0.0, 0.0, 0.0)
     chunks = -(-head.N // head.chunk)
     nv.LAUNCHES[0] += (head.N > COUNT_ROWS) + 2 * chunks

@@ -470,3 +470,27 @@ def test_more_than_two_to_the_31_logits():
     assert float((dx.double() - whole).norm() / whole.norm()) < BF16
     whole = sum(g[1].double() for g in grads)
     assert float((dw.double() - whole).norm() / whole.norm()) < 2 * BF16
+
+
+def test_no_room_for_logits(monkeypatch):
+    x, w, t, old, adv, ref = _setup(1032)
+    want = [torch.autograd.grad(_calls(x, w, t, old, adv, ref, 500)[k]()[0], [x, w]) for k in ("policy", "preference", "logprobs")]
+    real, refused = torch.empty, []
+
+    def empty(*shape, **kw):
+        if kw.get("dtype") == torch.uint8 and shape[0] >= 2 * x.shape[0] * x.shape[1] * 512 + x.numel() * 2:
+            refused.append(shape[0])
+            raise torch.OutOfMemoryError("no room")
+        return real(*shape, **kw)
+    monkeypatch.setattr(torch, "empty", empty)
+    got = []
+    for k in ("policy", "preference", "logprobs"):
+        outs = _calls(x, w, t, old, adv, ref, 500)[k]()
+        monkeypatch.setattr(torch, "empty", real)
+        got.append(torch.autograd.grad(outs[0], [x, w]))
+        monkeypatch.setattr(torch, "empty", empty)
+    assert len(refused) == 3
+    for a, b in zip(got, want):
+        for p, q in zip(a, b):
+            # each is rounded twice to bf16, of which the second time alone is at one place
+            assert float((p.double() - q.double()).norm() / q.double().norm()) < 4 * BF16
