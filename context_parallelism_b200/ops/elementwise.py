@@ -7,6 +7,7 @@ accumulated there in fp32.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -192,6 +193,11 @@ class _NormFn(torch.autograd.Function):
                 None, None)
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm_drop_parts(rows: int, d: int, layer: int) -> int:
+    return nv.lib().cpb_norm_drop_parts(rows, d, layer)
+
+
 class _NormDropFn(torch.autograd.Function):
     """``x_new = x + dropout(res)``, ``y = norm(x_new)``; returns ``(y, x_new)``.  No view is made or returned: on short rows the host
     takes longer than the GPU (136 x 768 forward and backward 167 us with the steps of ``_NormFn``, 138 like this)."""
@@ -224,8 +230,12 @@ class _NormDropFn(torch.autograd.Function):
         if any(own):
             buf = torch.zeros((sum(own), d), dtype=torch.float32, device=dy.device)
             dw, db = buf[0] if own[0] else dw, buf[-1] if own[1] else db
+        parts = None
+        if dw is not None or db is not None:                         # the blocks' sums, added in a launch of their own
+            parts = torch.empty(_norm_drop_parts(ctx.rows, d, ctx.layer), dtype=torch.float32, device=dy.device)
+            nv.LAUNCHES[0] += 1
         nv.call("norm_drop_bwd", xnew.data_ptr(), dy.data_ptr(), nv.ptr(dxnew), nv.ptr(wp), stats.data_ptr(), dx.data_ptr(), dres.data_ptr(),
-                nv.ptr(dw), nv.ptr(db), ctx.rows, d, ctx.layer, seed.data_ptr(), nv.ptr(pos), *ctx.place, nv.stream_ptr(dy.device))
+                nv.ptr(dw), nv.ptr(db), nv.ptr(parts), ctx.rows, d, ctx.layer, seed.data_ptr(), nv.ptr(pos), *ctx.place, nv.stream_ptr(dy.device))
         for prm in (wp, bp):
             hook = getattr(prm, "_grad_ready", None)
             if hook is not None:

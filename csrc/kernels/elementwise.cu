@@ -385,7 +385,8 @@ __device__ __forceinline__ void norm_bwd_rows(const __nv_bfloat16* __restrict__ 
       }
     }
   }
-  // the groups of a block are added in shared memory, the blocks in global memory.  One group: four columns per addition (one
+  // the groups of a block are added in shared memory, the blocks in global memory (DROP: every block has a place of its own there, and
+  // norm_params_kernel adds them in their order, so that the gradients repeat).  One group: four columns per addition (one
   // column at a time, 32 bytes from lane to lane, takes 33 us at 2048 x 1032, where 256 blocks meet on every column).
   for (int pass = 0; pass < (LAYER ? 2 : 1); ++pass) {
     float* dst = pass ? db : dw;
@@ -395,7 +396,10 @@ __device__ __forceinline__ void norm_bwd_rows(const __nv_bfloat16* __restrict__ 
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = pass ? ab[j] : aw[j];
-        if (((uintptr_t)dst & 15) == 0) {
+        if (DROP) {
+          ((float4*)dst)[2 * c] = make_float4(v[0], v[1], v[2], v[3]);
+          ((float4*)dst)[2 * c + 1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else if (((uintptr_t)dst & 15) == 0) {
           red_add_v4(dst + c * 8, v[0], v[1], v[2], v[3]);
           red_add_v4(dst + c * 8 + 4, v[4], v[5], v[6], v[7]);
         } else {
@@ -411,7 +415,8 @@ __device__ __forceinline__ void norm_bwd_rows(const __nv_bfloat16* __restrict__ 
       for (int i = threadIdx.x; i < d; i += TB) {
         float v = 0.f;
         for (int k = 0; k < NG; ++k) v += part[k * G * 8 + i];
-        atomicAdd(&dst[i], v);
+        if (DROP) dst[i] = v;
+        else atomicAdd(&dst[i], v);
       }
     }
   }
@@ -428,9 +433,31 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
 template <bool LAYER, int G>
 __global__ void __launch_bounds__(G > 256 ? 512 : 256, G > 256 ? 1 : 2)
 norm_drop_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ dres,
-                     const float* __restrict__ w, const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx, float* __restrict__ dw,
-                     float* __restrict__ db, int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
-  norm_bwd_rows<LAYER, G, true>(x, dy, dres, w, stats, dx, dw, db, rows, d, dbranch, q);
+                     const float* __restrict__ w, const float* __restrict__ stats, __nv_bfloat16* __restrict__ dx, float* __restrict__ parts,
+                     int rows, int d, __nv_bfloat16* __restrict__ dbranch, Drop q) {
+  float* mine = parts == nullptr ? nullptr : parts + (size_t)blockIdx.x * (LAYER ? 2 : 1) * d;
+  norm_bwd_rows<LAYER, G, true>(x, dy, dres, w, stats, dx, mine, mine == nullptr ? nullptr : mine + d, rows, d, dbranch, q);
+}
+// dw += and db += the blocks' parts [blocks][1 or 2][d], in their order.  32 columns per block, every eighth part for a warp.
+__global__ void __launch_bounds__(256)
+norm_params_kernel(const float* __restrict__ parts, float* __restrict__ dw, float* __restrict__ db, int blocks, int d) {
+  pdl_release();
+  pdl_wait();
+  __shared__ float sum[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float* dst = blockIdx.y ? db : dw;
+  const size_t step = (size_t)gridDim.y * d;
+  float v = 0.f;
+  if (c < d) {
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += 8) v += parts[b * step + (size_t)blockIdx.y * d + c];
+  }
+  sum[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || c >= d || dst == nullptr) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) v += sum[k][lane];
+  dst[c] += v;
 }
 
 // ============================================================================ activations (backward)
@@ -1187,10 +1214,19 @@ extern "C" int cpb_norm_bwd(const void* x, const void* dy, const void* dres, con
   return check_launch("norm_bwd");
 }
 
-// as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped
+static int norm_drop_blocks(int rows, int d) {
+  const int nvec = d / 8, G = nvec <= 32 ? 32 : nvec <= 64 ? 64 : nvec <= 128 ? 128 : nvec <= 256 ? 256 : 512, tb = G > 256 ? 512 : 256;
+  const int per_block = norm_bwd_turn(true) * (tb / G), cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block;
+  return need < cap ? need : cap;
+}
+// Floats of the workspace of cpb_norm_drop_bwd.
+extern "C" int cpb_norm_drop_parts(int rows, int d, int layer) { return rows <= 0 ? 0 : norm_drop_blocks(rows, d) * (layer ? 2 : 1) * d; }
+
+// as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped.  parts: workspace, needed for dw and db.
 extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, void* dbranch,
-                                 float* dw, float* db, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T, long seq_len, long site,
-                                 double p, cudaStream_t stream) {
+                                 float* dw, float* db, float* parts, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T,
+                                 long seq_len, long site, double p, cudaStream_t stream) {
+  if ((dw != nullptr || db != nullptr) && (parts == nullptr || ((uintptr_t)parts & 15))) return set_error(CPB_ERR_ARG, "norm: gradients of parameters need a workspace");
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
   const int nvec = d / 8;
@@ -1199,17 +1235,19 @@ extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres
   const int rc = make_drop(q, seed, pos, rows, T, seq_len, site, p);
   if (rc != CPB_OK) return rc;
   if (dbranch == nullptr) return set_error(CPB_ERR_ARG, "norm: dropout needs the branch's gradient");
+  const int blocks = norm_drop_blocks(rows, d);
 #define NORM_BWD(G)                                                                                                             \
   do {                                                                                                                          \
-    const int tb = G > 256 ? 512 : 256, R = norm_bwd_turn(true), per_block = R * (tb / G), smem = 2 * 3 * R * 16 * tb;          \
-    const int cap = sm_count() * (G > 256 ? 1 : 2), need = (rows + per_block - 1) / per_block, blocks = need < cap ? need : cap; \
+    const int tb = G > 256 ? 512 : 256, smem = 2 * 3 * norm_bwd_turn(true) * 16 * tb;                                           \
     auto kern = layer ? norm_drop_bwd_kernel<true, G> : norm_drop_bwd_kernel<false, G>;                                         \
     CPB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));                                 \
     CPB_CUDA_OK(launch_pdl(kern, blocks, tb, smem, stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)dy, (const __nv_bfloat16*)dres, w, stats, \
-                                    (__nv_bfloat16*)dx, dw, db, rows, d, (__nv_bfloat16*)dbranch, q));                           \
+                                    (__nv_bfloat16*)dx, parts, rows, d, (__nv_bfloat16*)dbranch, q));                            \
   } while (0)
   NORM_GROUPS(NORM_BWD);
 #undef NORM_BWD
+  if (parts != nullptr)
+    CPB_CUDA_OK(launch_pdl(norm_params_kernel, dim3((d + 31) / 32, layer ? 2 : 1), 256, 0, stream, (const float*)parts, dw, db, blocks, d));
   return check_launch("norm_drop_bwd");
 }
 

@@ -34,7 +34,7 @@ def _pos(kind, T):
 
 
 # every width class of the norms' kernels, single rows, odd numbers of rows
-SHAPES = [(1, 1, 8), (1, 3, 64), (2, 33, 264), (3, 17, 384), (1, 136, 768), (4, 5, 1032), (2, 129, 2048), (1, 9, 2056), (1, 40, 4096), (131, 512)]
+SHAPES = [(3, 1001, 64), (1, 2500, 520), (1, 1, 8), (1, 3, 64), (2, 33, 264), (3, 17, 384), (1, 136, 768), (4, 5, 1032), (2, 129, 2048), (1, 9, 2056), (1, 40, 4096), (131, 512)]
 
 
 @pytest.mark.parametrize("kind", ["whole", "shard", "far"])
@@ -67,6 +67,9 @@ def test_norms(shape, norm, p, kind):
     leaves = [x, r, w] + ([b] if layer else [])
     dx, dr, *dw = torch.autograd.grad([y, new], leaves, [dy, dnew])
     scale = 1 / (1 - p)
+    again = E.layernorm(x, w, b, 1e-5, r, drop) if layer else E.rmsnorm(x, w, 1e-5, r, drop)
+    for p1, p2 in zip((y, new, dx, dr, *dw), (*again, *torch.autograd.grad(again, leaves, [dy, dnew]))):
+        assert torch.equal(p1, p2)                                   # bit for bit
     assert torch.equal(new, (x.float() + torch.where(keep, r.float() * scale, 0.0)).bfloat16())
     v = new.detach().double().requires_grad_()
     W, B = w.detach().double().requires_grad_(), b.detach().double().requires_grad_()
@@ -185,3 +188,24 @@ def test_recorded_evaluation_drops_nothing():
         x, y, pos = a.shard_batch(*_batch(a, i))
         a.forward_backward(*_batch(a, i))
         assert torch.equal(a.model.per_token_nll(x, y, pos), b.model.per_token_nll(x, y, pos))
+
+
+def test_parameters_add_to_what_is_there():
+    gen, drop, _ = _case((2, 50, 256), 0.2)
+    x, r, dy = (_randn(gen, 2, 50, 256) for _ in range(3))
+    x.requires_grad_()
+    grads = []
+    for main in (False, True):
+        w, b = (torch.ones(256, device="cuda", requires_grad=True) for _ in range(2))
+        told = []
+        if main:
+            w.main_grad, b.main_grad = (torch.full((256,), 2.0, device="cuda") for _ in range(2))
+            w._grad_ready = b._grad_ready = told.append
+        y, _ = E.layernorm(x, w, b, 1e-5, r, drop)
+        y.backward(dy)
+        grads.append([w.main_grad - 2.0, b.main_grad - 2.0] if main else [w.grad, b.grad])
+        assert len(told) == 2 * main
+    for p, q in zip(*grads):
+        assert float((p - q).abs().max()) <= 2.0 ** -24 * (4 + 2 * float(p.abs().max()))        # added to two and taken from it again
+    y, _ = E.rmsnorm(x, None, 1e-5, r, drop)                          # no parameters at all
+    y.backward(dy)
