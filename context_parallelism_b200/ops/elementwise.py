@@ -11,6 +11,7 @@ import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native as nv
 from . import reference as ref
@@ -105,6 +106,7 @@ class _DropoutFn(torch.autograd.Function):
         return _dropout(x, drop)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         seed, pos = ctx.saved_tensors
         return _dropout(dy, ctx.drop._replace(seed=seed, pos=pos)), None, None, None
@@ -219,6 +221,7 @@ class _NormDropFn(torch.autograd.Function):
         return y, xnew
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dxnew):
         xnew, stats, seed, pos = ctx.saved_tensors
         wp, bp, d = ctx.w, ctx.b, xnew.shape[-1]
@@ -259,7 +262,10 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor], eps: float, residual: Op
     """Returns ``(rmsnorm(x + residual) * w, x + residual)``; with ``drop``, ``dropout(residual, drop)`` in the place of ``residual``."""
     drop = _branch_drop(x, residual, drop)
     if x.is_cuda:
-        return _NormFn.apply(x, residual, w, None, eps, 0) if drop is None else _NormDropFn.apply(x, residual, w, None, eps, 0, drop)
+        if drop is None:
+            return _NormFn.apply(x, residual, w, None, eps, 0)
+        with nv.on(x.device):
+            return _NormDropFn.apply(x, residual, w, None, eps, 0, drop)
     xn = x if residual is None else x + (residual if drop is None else ref.dropout(residual, drop))
     return ref.rmsnorm(xn, w, eps), xn
 
@@ -268,7 +274,10 @@ def layernorm(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], eps: 
               residual: Optional[torch.Tensor] = None, drop: Optional[Dropout] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     drop = _branch_drop(x, residual, drop)
     if x.is_cuda:
-        return _NormFn.apply(x, residual, w, b, eps, 1) if drop is None else _NormDropFn.apply(x, residual, w, b, eps, 1, drop)
+        if drop is None:
+            return _NormFn.apply(x, residual, w, b, eps, 1)
+        with nv.on(x.device):
+            return _NormDropFn.apply(x, residual, w, b, eps, 1, drop)
     xn = x if residual is None else x + (residual if drop is None else ref.dropout(residual, drop))
     return ref.layernorm(xn, w, b, eps), xn
 

@@ -8,7 +8,7 @@ cross entropy in two ways: tokens that count are gathered before the products, a
 gradient may come in and a loss that is never differentiated costs no more than its forward pass.
 
 Each takes what the head's GEMM takes: bf16 ``x`` and ``w`` on one GPU, ``d`` and ``V`` multiples of 8.  ``n_valid``: rows of ``w`` from there on
-are padding.  Gradients of ``w`` are added to ``w.main_grad`` when it has one.  Nothing waits for the GPU, and all calls can be captured.
+are padding, with finite numbers in them.  Gradients of ``w`` are added to ``w.main_grad`` when it has one.  Nothing waits for the GPU, and all calls can be captured.
 CPU tensors take the plain form."""
 from __future__ import annotations
 

@@ -1226,9 +1226,9 @@ extern "C" int cpb_norm_drop_parts(int rows, int d, int layer) { return rows <= 
 extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, void* dbranch,
                                  float* dw, float* db, float* parts, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T,
                                  long seq_len, long site, double p, cudaStream_t stream) {
-  if ((dw != nullptr || db != nullptr) && (parts == nullptr || ((uintptr_t)parts & 15))) return set_error(CPB_ERR_ARG, "norm: gradients of parameters need a workspace");
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
+  if ((dw != nullptr || db != nullptr) && (parts == nullptr || ((uintptr_t)parts & 15))) return set_error(CPB_ERR_ARG, "norm: gradients of parameters need a workspace");
   const int nvec = d / 8;
   if (nvec > 512) return set_error(CPB_ERR_LIMIT, "norm: d=%d exceeds 4096", d);
   Drop q;

@@ -209,3 +209,22 @@ def test_parameters_add_to_what_is_there():
         assert float((p - q).abs().max()) <= 2.0 ** -24 * (4 + 2 * float(p.abs().max()))        # added to two and taken from it again
     y, _ = E.rmsnorm(x, None, 1e-5, r, drop)                          # no parameters at all
     y.backward(dy)
+
+
+def test_no_rows_through_a_norm():
+    drop = E.Dropout(0.1, torch.tensor([1], device="cuda"))
+    x, r = (torch.zeros(2, 0, 64, device="cuda", dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    w, b = (torch.ones(64, device="cuda", requires_grad=True) for _ in range(2))
+    y, new = E.layernorm(x, w, b, 1e-5, r, drop)
+    assert y.shape == new.shape == x.shape
+    (y.sum() + new.sum()).backward()
+    assert x.grad.shape == r.grad.shape == x.shape and not bool(w.grad.any()) and not bool(b.grad.any())
+
+
+def test_second_derivatives_are_refused():
+    gen, drop, _ = _case((2, 5, 64), 0.2)
+    x, r, dy = (_randn(gen, 2, 5, 64).requires_grad_() for _ in range(3))
+    for y in (E.dropout(x, drop), E.rmsnorm(x, None, 1e-5, r, drop)[0]):
+        dx, = torch.autograd.grad(y, x, dy, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.float().sum().backward()
