@@ -231,14 +231,14 @@ class _NormDropFn(torch.autograd.Function):
         dw, db = getattr(wp, "main_grad", None), getattr(bp, "main_grad", None)
         own = [p is not None and g is None for p, g in ((wp, dw), (bp, db))]
         if any(own):
-            buf = torch.zeros((sum(own), d), dtype=torch.float32, device=dy.device)
+            buf = (torch.empty if ctx.rows else torch.zeros)((sum(own), d), dtype=torch.float32, device=dy.device)
             dw, db = buf[0] if own[0] else dw, buf[-1] if own[1] else db
         parts = None
         if dw is not None or db is not None:                         # the blocks' sums, added in a launch of their own
             parts = torch.empty(_norm_drop_parts(ctx.rows, d, ctx.layer), dtype=torch.float32, device=dy.device)
             nv.LAUNCHES[0] += 1
         nv.call("norm_drop_bwd", xnew.data_ptr(), dy.data_ptr(), nv.ptr(dxnew), nv.ptr(wp), stats.data_ptr(), dx.data_ptr(), dres.data_ptr(),
-                nv.ptr(dw), nv.ptr(db), nv.ptr(parts), ctx.rows, d, ctx.layer, seed.data_ptr(), nv.ptr(pos), *ctx.place, nv.stream_ptr(dy.device))
+                nv.ptr(dw), nv.ptr(db), 2 * (not own[1]) + (not own[0]), nv.ptr(parts), ctx.rows, d, ctx.layer, seed.data_ptr(), nv.ptr(pos), *ctx.place, nv.stream_ptr(dy.device))
         for prm in (wp, bp):
             hook = getattr(prm, "_grad_ready", None)
             if hook is not None:

@@ -438,9 +438,10 @@ norm_drop_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* _
   float* mine = parts == nullptr ? nullptr : parts + (size_t)blockIdx.x * (LAYER ? 2 : 1) * d;
   norm_bwd_rows<LAYER, G, true>(x, dy, dres, w, stats, dx, mine, mine == nullptr ? nullptr : mine + d, rows, d, dbranch, q);
 }
-// dw += and db += the blocks' parts [blocks][1 or 2][d], in their order.  32 columns per block, every eighth part for a warp.
+// The blocks' parts [blocks][1 or 2][d], in their order: written to dw and db, or added where a bit of `add` is set (1 dw, 2 db).  32 columns per block, every
+// eighth part for a warp; 3 us.
 __global__ void __launch_bounds__(256)
-norm_params_kernel(const float* __restrict__ parts, float* __restrict__ dw, float* __restrict__ db, int blocks, int d) {
+norm_params_kernel(const float* __restrict__ parts, float* __restrict__ dw, float* __restrict__ db, int add, int blocks, int d) {
   pdl_release();
   pdl_wait();
   __shared__ float sum[8][32];
@@ -457,7 +458,7 @@ norm_params_kernel(const float* __restrict__ parts, float* __restrict__ dw, floa
   if (warp != 0 || c >= d || dst == nullptr) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) v += sum[k][lane];
-  dst[c] += v;
+  dst[c] = add >> blockIdx.y & 1 ? dst[c] + v : v;
 }
 
 // ============================================================================ activations (backward)
@@ -1222,9 +1223,10 @@ static int norm_drop_blocks(int rows, int d) {
 // Floats of the workspace of cpb_norm_drop_bwd.
 extern "C" int cpb_norm_drop_parts(int rows, int d, int layer) { return rows <= 0 ? 0 : norm_drop_blocks(rows, d) * (layer ? 2 : 1) * d; }
 
-// as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped.  parts: workspace, needed for dw and db.
+// as well dbranch = drop(dx), the gradient of the branch that cpb_norm_drop_fwd has dropped.  parts: workspace, needed for dw and db, which are written or, with
+// bits 1 and 2 of `add`, added to.
 extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres, const float* w, const float* stats, void* dx, void* dbranch,
-                                 float* dw, float* db, float* parts, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T,
+                                 float* dw, float* db, int add, float* parts, int rows, int d, int layer, const int64_t* seed, const int64_t* pos, int T,
                                  long seq_len, long site, double p, cudaStream_t stream) {
   if (d % 8) return set_error(CPB_ERR_ARG, "norm: d=%d must be a multiple of 8", d);
   if (rows <= 0) return CPB_OK;
@@ -1247,7 +1249,7 @@ extern "C" int cpb_norm_drop_bwd(const void* x, const void* dy, const void* dres
   NORM_GROUPS(NORM_BWD);
 #undef NORM_BWD
   if (parts != nullptr)
-    CPB_CUDA_OK(launch_pdl(norm_params_kernel, dim3((d + 31) / 32, layer ? 2 : 1), 256, 0, stream, (const float*)parts, dw, db, blocks, d));
+    CPB_CUDA_OK(launch_pdl(norm_params_kernel, dim3((d + 31) / 32, layer ? 2 : 1), 256, 0, stream, (const float*)parts, dw, db, add, blocks, d));
   return check_launch("norm_drop_bwd");
 }
 

@@ -195,17 +195,17 @@ def test_parameters_add_to_what_is_there():
     x, r, dy = (_randn(gen, 2, 50, 256) for _ in range(3))
     x.requires_grad_()
     grads = []
-    for main in (False, True):
-        w, b = (torch.ones(256, device="cuda", requires_grad=True) for _ in range(2))
+    for main in ((), (0, 1), (0,), (1,)):
+        w, b = both = [torch.ones(256, device="cuda", requires_grad=True) for _ in range(2)]
         told = []
-        if main:
-            w.main_grad, b.main_grad = (torch.full((256,), 2.0, device="cuda") for _ in range(2))
-            w._grad_ready = b._grad_ready = told.append
+        for i in main:
+            both[i].main_grad = torch.full((256,), 2.0, device="cuda")
+            both[i]._grad_ready = told.append
         y, _ = E.layernorm(x, w, b, 1e-5, r, drop)
         y.backward(dy)
-        grads.append([w.main_grad - 2.0, b.main_grad - 2.0] if main else [w.grad, b.grad])
-        assert len(told) == 2 * main
-    for p, q in zip(*grads):
+        grads.append([both[i].main_grad - 2.0 if i in main else both[i].grad for i in range(2)])
+        assert len(told) == len(main)
+    for p, q in ((p, q) for other in grads[1:] for p, q in zip(grads[0], other)):
         assert float((p - q).abs().max()) <= 2.0 ** -24 * (4 + 2 * float(p.abs().max()))        # added to two and taken from it again
     y, _ = E.rmsnorm(x, None, 1e-5, r, drop)                          # no parameters at all
     y.backward(dy)
