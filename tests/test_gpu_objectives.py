@@ -494,3 +494,18 @@ def test_no_room_for_logits(monkeypatch):
         for p, q in zip(a, b):
             # each is rounded twice to bf16, of which the second time alone is at one place
             assert float((p.double() - q.double()).norm() / q.double().norm()) < 4 * BF16
+
+
+# more rows than one launch takes: 65280
+@pytest.mark.parametrize("B,T,d,V,n_valid,spans", [(1, 70001, 64, 264, 260, "scattered"), (3, 40000, 520, 128, 128, "response"), (1, 66000, 128, 64, 60, "65281"),
+                                                   (1, 66000, 128, 64, 60, "3"), (70000, 2, 8, 16, 16, "none")])
+def test_more_rows_than_a_launch_takes(B, T, d, V, n_valid, spans):
+    assert B * T > O._chunk(V)
+    test_logprobs(B, T, d, V, n_valid, spans, None)
+    if spans != "none":
+        test_policy(B, T, d, V, n_valid, spans, 0.3, (0.2, 0.28), None)
+
+
+@pytest.mark.parametrize("B,T,d", [(65534, 1, 64), (3000, 7, 520), (2, 70000, 64)])
+def test_many_pairs_and_long_ones(B, T, d):
+    test_preference(B, T, d, 64, 60, "scattered", 0.1, 0.3, None)
